@@ -19,6 +19,7 @@
 
 #include "../../include/goinfer_cuda.h"
 #include "batch_alias.h"
+#include "capi.cuh"
 #include "gemm.cuh"
 #include "gemv.cuh"
 #include "model.cuh"
@@ -441,6 +442,21 @@ int layer_refs(const gi_cuda_layer_weights_t* lw, uint32_t n_layers, int64_t dim
 }
 
 }  // namespace
+
+namespace gi {
+
+std::mutex& capi_mutex() { return g.mu; }
+
+int capi_ready(CapiCtx* c) {
+  if (int rc = ensure_ready()) return rc;
+  c->sm_count = g.sm_count;
+  c->stream = g.stream;
+  return 0;
+}
+
+int capi_fail(int code, const char* what, cudaError_t e) { return fail(code, what, e); }
+
+}  // namespace gi
 
 // Fixed device scratch of gi_cuda_gemm_dev_noalloc: the prefill workspace
 // (staged fp16 activation tiles, sub-block sums, per-token scales) lives in

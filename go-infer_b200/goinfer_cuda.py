@@ -29,6 +29,7 @@ LIB_PATH = os.path.join(HERE, "libgoinfer_cuda.so")
 
 # GGML type ids, pkg/gguf/types.go:25-52
 TYPE_F32 = 0
+TYPE_F16 = 1  # KV caches only
 TYPE_Q8_0 = 8
 TYPE_Q4_K = 12
 TYPE_Q6_K = 14
@@ -53,6 +54,8 @@ EXPORTS = (
     "gi_cuda_alloc_buffers", "gi_cuda_forward_transformer", "gi_cuda_model_create", "gi_cuda_model_destroy",
     "gi_cuda_model_reset", "gi_cuda_model_set_persistent", "gi_cuda_model_generate", "gi_cuda_tp_prepare", "gi_cuda_tp_connect", "gi_cuda_tp_close",
     "gi_cuda_alloc_buffer", "gi_synth_weights", "gi_cuda_buffer_read",
+    "gi_kv_cache_bytes", "gi_rope_freqs", "gi_cuda_kv_write_dev", "gi_cuda_kv_read_dev", "gi_cuda_attn_workspace",
+    "gi_cuda_attn_dev", "gi_cuda_sample_dev",
 )
 
 
@@ -80,6 +83,25 @@ class ModelDesc(ctypes.Structure):
                 ("output_norm", ctypes.c_void_p),
                 ("output_weight", ctypes.c_void_p), ("output_weight_type", ctypes.c_int),
                 ("tp_world", ctypes.c_uint32), ("tp_rank", ctypes.c_uint32), ("vocab_offset", ctypes.c_uint32)]
+
+
+class KVCacheDesc(ctypes.Structure):
+    """gi_cuda_kv_cache_t."""
+    _fields_ = [("type", ctypes.c_int), ("n_pages", ctypes.c_uint32), ("page_size", ctypes.c_uint32),
+                ("n_kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("data", ctypes.c_void_p),
+                ("bytes", ctypes.c_size_t)]
+
+
+class RopeDesc(ctypes.Structure):
+    """gi_cuda_rope_t."""
+    _fields_ = [("dim", ctypes.c_uint32), ("interleaved", ctypes.c_int), ("freqs", ctypes.c_void_p),
+                ("mscale", ctypes.c_double)]
+
+
+class AttnDesc(ctypes.Structure):
+    """gi_cuda_attn_t."""
+    _fields_ = [("n_heads", ctypes.c_uint32), ("max_tokens", ctypes.c_uint32), ("max_q_len", ctypes.c_uint32),
+                ("prefix_len", ctypes.c_uint32), ("scale", ctypes.c_float)]
 
 
 class GoInferCudaError(RuntimeError):
@@ -154,6 +176,16 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "gi_cuda_model_set_persistent": ([vp, i32], i32),
         "gi_cuda_model_generate": ([vp, ctypes.POINTER(ctypes.c_int32), u32, u32, u32, ctypes.POINTER(u32), f32p,
                                     f32p], i32),
+    }
+    i64, f64 = ctypes.c_int64, ctypes.c_double
+    sig |= {
+        "gi_kv_cache_bytes": ([i32, u32, u32, u32, u32], i64),
+        "gi_rope_freqs": ([i32, u32, f64, f64, f64, f64, f64, vp, ctypes.POINTER(f64)], i32),
+        "gi_cuda_kv_write_dev": ([vp, vp, sz, vp, sz, vp, u32, vp, sz, vp, u32, vp, vp, vp], i32),
+        "gi_cuda_kv_read_dev": ([vp, vp, vp, vp, u32, vp], i32),
+        "gi_cuda_attn_workspace": ([vp, vp], i64),
+        "gi_cuda_attn_dev": ([vp, vp, vp, vp, u32, u32, vp, vp, vp, u32, vp, vp, sz, vp], i32),
+        "gi_cuda_sample_dev": ([vp, vp, vp, sz, u32, u32, vp, vp, vp, vp, vp, vp], i32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
@@ -398,6 +430,112 @@ def quantize(quant_type: int, src: np.ndarray, threads: int = 0) -> np.ndarray:
     _err("gi_quantize", load_library().gi_quantize(quant_type, _f32(src), rows, cols,
                                                     ctypes.c_void_p(out.ctypes.data), threads))
     return out
+
+
+# ---- serving a batch from a paged KV cache ---------------------------------
+# Device pointers (ints) and streams as above; see include/goinfer_cuda.h for
+# what each call reads and writes.
+
+ROPE_NONE, ROPE_LINEAR, ROPE_LLAMA3, ROPE_YARN = range(4)
+
+
+class KVCache:
+    """A layer's paged F16 or Q8_0 cache: in memory of the caller's
+    (data_ptr, nbytes; 256-byte aligned) or in a Buffer of its own."""
+
+    def __init__(self, type: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, data_ptr: int = 0,
+                 nbytes: int = 0):
+        need = int(load_library().gi_kv_cache_bytes(type, n_pages, page_size, n_kv_heads, head_dim))
+        if need < 0:
+            raise GoInferCudaError("gi_kv_cache_bytes", ERR_SHAPE, "unsupported cache type or shape")
+        self.buf: Optional[Buffer] = None
+        if not data_ptr:
+            h = load_library().gi_cuda_alloc_buffer(need)
+            if not h:
+                raise GoInferCudaError("gi_cuda_alloc_buffer", ERR_BUFFER,
+                                       load_library().gi_cuda_last_error().decode(errors="replace"))
+            self.buf = Buffer(h, need)
+            data_ptr, nbytes = self.buf.device_ptr, need
+        self.type, self.n_pages, self.page_size = type, n_pages, page_size
+        self.n_kv_heads, self.head_dim, self.nbytes = n_kv_heads, head_dim, nbytes
+        self.desc = KVCacheDesc(type, n_pages, page_size, n_kv_heads, head_dim, data_ptr, nbytes)
+        self._p = ctypes.addressof(self.desc)
+
+    def close(self) -> None:
+        ReleaseBuffer(self.buf)
+        self.buf = None
+
+
+def rope_freqs(dim: int, theta: float, scaling: int = ROPE_NONE, factor: float = 1.0, low: float = 1.0,
+               high: float = 4.0, orig_ctx: float = 8192.0) -> tuple[np.ndarray, float]:
+    """(dim / 2 float64 frequencies, factor on cos and sin) for Rope."""
+    out = np.empty(max(dim // 2, 1), np.float64)
+    m = ctypes.c_double(1.0)
+    _err("gi_rope_freqs", load_library().gi_rope_freqs(scaling, dim, theta, factor, low, high, orig_ctx,
+                                                       out.ctypes.data, ctypes.byref(m)))
+    return out, m.value
+
+
+class Rope:
+    """Rotary positions of the first `dim` values of a head; freqs_ptr: dim / 2 doubles on the device."""
+
+    def __init__(self, dim: int, freqs_ptr: int, interleaved: bool = False, mscale: float = 1.0):
+        self.desc = RopeDesc(dim, int(interleaved), freqs_ptr, mscale)
+        self._p = ctypes.addressof(self.desc)
+
+
+def kv_write_dev(cache: KVCache, k_ptr: int, v_ptr: int, slots_ptr: int, n_tokens: int, *, k_stride: int = 0,
+                 v_stride: int = 0, q_ptr: int = 0, q_out_ptr: int = 0, heads: int = 0, q_stride: int = 0,
+                 positions_ptr: int = 0, rope: Optional[Rope] = None, stream: int = 0) -> None:
+    """Rotates q into q_out and k into the cache and writes v (strides in floats; 0: rows back to back)."""
+    row = cache.n_kv_heads * cache.head_dim
+    rc = (_lib or load_library()).gi_cuda_kv_write_dev(
+        cache._p, k_ptr, k_stride or row, v_ptr, v_stride or row, slots_ptr, n_tokens, q_ptr or None,
+        q_stride or heads * cache.head_dim, q_out_ptr or None, heads, positions_ptr or None, rope._p if rope else None,
+        stream or None)
+    if rc:
+        _err("gi_cuda_kv_write_dev", rc)
+
+
+def kv_read_dev(cache: KVCache, k_ptr: int, v_ptr: int, slots_ptr: int, n_tokens: int, stream: int = 0) -> None:
+    """The cached rows of the slots as float32 [n_tokens][n_kv_heads][head_dim]."""
+    rc = (_lib or load_library()).gi_cuda_kv_read_dev(cache._p, k_ptr, v_ptr, slots_ptr, n_tokens, stream or None)
+    if rc:
+        _err("gi_cuda_kv_read_dev", rc)
+
+
+class Attention:
+    """Attention calls of one description over one cache; workspace_bytes is what each call needs."""
+
+    def __init__(self, cache: KVCache, *, heads: int, max_tokens: int, max_q_len: int = 1, scale: float,
+                 prefix_len: int = 0):
+        self.cache = cache
+        self.desc = AttnDesc(heads, max_tokens, max_q_len, prefix_len, scale)
+        self._p = ctypes.addressof(self.desc)
+        n = int(load_library().gi_cuda_attn_workspace(cache._p, self._p))
+        if n < 0:
+            _err("gi_cuda_attn_workspace", n)
+        self.workspace_bytes = n
+
+    def __call__(self, out_ptr: int, q_ptr: int, n_seqs: int, n_tokens: int, kv_len_ptr: int, pages_ptr: int,
+                 pages_stride: int, workspace_ptr: int, workspace_bytes: int, *, q_start_ptr: int = 0,
+                 prefix_pages_ptr: int = 0, stream: int = 0) -> None:
+        rc = _lib.gi_cuda_attn_dev(self.cache._p, self._p, out_ptr, q_ptr, n_seqs, n_tokens, q_start_ptr or None,
+                                   kv_len_ptr, pages_ptr, pages_stride, prefix_pages_ptr or None,
+                                   workspace_ptr or None, workspace_bytes, stream or None)
+        if rc:
+            _err("gi_cuda_attn_dev", rc)
+
+
+def sample_dev(ids_ptr: int, logits_ptr: int, rows: int, vocab: int, u_ptr: int, *, temperature_ptr: int = 0,
+               top_k_ptr: int = 0, top_p_ptr: int = 0, min_p_ptr: int = 0, prob_ptr: int = 0, logits_stride: int = 0,
+               stream: int = 0) -> None:
+    """The next token of each row of logits by its uniform number (logits_stride in floats; 0: vocab)."""
+    rc = (_lib or load_library()).gi_cuda_sample_dev(
+        ids_ptr, prob_ptr or None, logits_ptr, logits_stride or vocab, rows, vocab, u_ptr, temperature_ptr or None,
+        top_k_ptr or None, top_p_ptr or None, min_p_ptr or None, stream or None)
+    if rc:
+        _err("gi_cuda_sample_dev", rc)
 
 
 # ---- pkg/engine/weights.go dispatch mirror --------------------------------

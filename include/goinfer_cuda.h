@@ -41,6 +41,7 @@ extern "C" {
 
 /* GGML quant type ids, pkg/gguf/types.go:25-52. */
 #define GI_TYPE_F32 0
+#define GI_TYPE_F16 1 /* KV caches only */
 #define GI_TYPE_Q8_0 8
 #define GI_TYPE_Q4_K 12
 #define GI_TYPE_Q6_K 14
@@ -357,6 +358,131 @@ gi_cuda_buffer_t gi_cuda_alloc_buffer(size_t bytes);
  * Returns when the buffer is written. */
 int gi_synth_weights(gi_cuda_buffer_t buf, int quant_type, uint64_t seed, float stddev, int64_t row0, int64_t rows,
                      int64_t col0, int64_t cols);
+
+/* ---- serving a batch from a paged KV cache -----------------------------------
+ * What lies between the projections of a batch of tokens (gi_cuda_gemm_dev)
+ * and its next tokens: rotary positions, the cache as it is written and read
+ * back, attention over it, and sampling.  The device counterparts of
+ * pkg/engine/kvcache.go, paged_kv.go and prefix_cache.go, of
+ * metal_kv_write_batch and metal_attention_gqa_batch, and of pkg/sampler.
+ *
+ * All array arguments are device pointers (host arguments are the structs
+ * themselves), rows of float32 16-byte aligned.  The calls are asynchronous on
+ * `stream` (NULL = library stream), allocate nothing, never wait for the
+ * device and can be captured; lengths, positions, slots and pages are read on
+ * the device when the call runs, so a captured call follows them.  Indexes
+ * that lie outside their range are never followed: such a slot is skipped,
+ * the positions of such a page are not seen. */
+
+/* A layer's cache: n_pages pages of page_size positions (a power of two from
+ * 16 to 65536) of n_kv_heads heads of head_dim values (a multiple of 32 up to
+ * 256).  type: GI_TYPE_F16, or GI_TYPE_Q8_0 (int8 codes with one fp16 scale per
+ * 32 values by gi_quantize's rule; a value is code * scale rounded to half
+ * precision).  data: gi_kv_cache_bytes bytes, 256-byte aligned: the K values
+ * [page][kv head][offset][head_dim], the V values, the K scales
+ * [page][kv head][offset][head_dim / 32] and the V scales (Q8_0 only), each
+ * part starting on a multiple of 256 bytes.  Position p of a sequence lies in
+ * slot pages[p / page_size] * page_size + p % page_size. */
+typedef struct {
+  int type;
+  uint32_t n_pages, page_size, n_kv_heads, head_dim;
+  void* data;
+  size_t bytes;
+} gi_cuda_kv_cache_t;
+
+/* Size of a cache's data, or -1 for a type or shape that is not supported. */
+int64_t gi_kv_cache_bytes(int type, uint32_t n_pages, uint32_t page_size, uint32_t n_kv_heads, uint32_t head_dim);
+
+/* Rotary positions: the first `dim` values of a head (even, at most head_dim)
+ * turn by pos * freqs[i], pair i being (x[i], x[i + dim/2]) (kernels.go:22-36)
+ * or, interleaved, (x[2i], x[2i + 1]).  freqs: dim / 2 doubles on the
+ * device; mscale multiplies the cosines and sines. */
+typedef struct {
+  uint32_t dim;
+  int interleaved;
+  const double* freqs;
+  double mscale;
+} gi_cuda_rope_t;
+
+/* Frequencies for gi_cuda_rope_t, on the host: freqs[i] = theta^(-2i/dim),
+ * scaled for contexts longer than the model was trained on.  GI_ROPE_LINEAR
+ * divides by `factor`.  GI_ROPE_LLAMA3 divides the frequencies whose
+ * wavelength exceeds orig_ctx / low, keeps those below orig_ctx / high and
+ * blends between (low < high).  GI_ROPE_YARN divides those that turn fewer
+ * than `low` times within orig_ctx, keeps those that turn more than `high`
+ * times, blends between by pair index, and sets *mscale to
+ * 0.1 ln(factor) + 1.  *mscale is 1 otherwise. */
+#define GI_ROPE_NONE 0
+#define GI_ROPE_LINEAR 1
+#define GI_ROPE_LLAMA3 2
+#define GI_ROPE_YARN 3
+int gi_rope_freqs(int scaling, uint32_t dim, double theta, double factor, double low, double high, double orig_ctx,
+                  double* freqs, double* mscale);
+
+/* Rotates q into q_out and k into the cache, and writes v beside it, for
+ * n_tokens tokens.  Token t's rows are q + t * q_stride (n_heads heads; the
+ * strides count floats and are multiples of 4), k + t * k_stride and
+ * v + t * v_stride; q_out is [n_tokens][n_heads][head_dim] and may not
+ * overlap q.  slots[t] is where K and V go; a slot outside the cache (-1
+ * for a padding token) is not written, and no slot may appear twice.  q may be
+ * NULL (n_heads is then ignored); rope may be NULL: nothing turns, positions
+ * is not read. */
+int gi_cuda_kv_write_dev(const gi_cuda_kv_cache_t* cache, const float* k, size_t k_stride, const float* v,
+                         size_t v_stride, const int32_t* slots, uint32_t n_tokens, const float* q, size_t q_stride,
+                         float* q_out, uint32_t n_heads, const int32_t* positions, const gi_cuda_rope_t* rope,
+                         void* stream);
+
+/* The cached rows of n_tokens slots as float32: k and v are
+ * [n_tokens][n_kv_heads][head_dim]; the rows of a slot outside the cache
+ * are left as they are.  A slot may appear any number of times. */
+int gi_cuda_kv_read_dev(const gi_cuda_kv_cache_t* cache, float* k, float* v, const int32_t* slots, uint32_t n_tokens,
+                        void* stream);
+
+/* What an attention call's kernels and workspace are chosen by: n_heads query
+ * heads (a multiple of the cache's n_kv_heads); at most max_tokens tokens in
+ * a call and max_q_len of one sequence (choices follow max_q_len, results do not
+ * depend on it); prefix_len positions that every sequence sees before its
+ * own; scale on q.k. */
+typedef struct {
+  uint32_t n_heads, max_tokens, max_q_len, prefix_len;
+  float scale;
+} gi_cuda_attn_t;
+
+/* Workspace bytes of gi_cuda_attn_dev, or a negative status.  Calls that may
+ * run at the same time need a workspace each; its contents need not be kept
+ * or initialised. */
+int64_t gi_cuda_attn_workspace(const gi_cuda_kv_cache_t* cache, const gi_cuda_attn_t* attn);
+
+/* Attention of a ragged batch over the cache, head h with kv head
+ * h / (n_heads / n_kv_heads).  Sequence b's tokens are rows
+ * q_start[b] .. q_start[b + 1] - 1 of q and out ([n_tokens][n_heads][head_dim],
+ * q_start ascending; NULL: row b alone, n_tokens = n_seqs); they are the last
+ * of its kv_len[b] positions, which lie in pages[b * pages_stride ...] and are
+ * in the cache already.  A token sees the prefix (prefix_pages; NULL when
+ * prefix_len is 0) and its sequence's positions up to its own.  A row that sees
+ * nothing is 0; rows behind the last sequence are left as they are.  Positions
+ * that a sequence does not have are not read, whatever their pages hold. */
+int gi_cuda_attn_dev(const gi_cuda_kv_cache_t* cache, const gi_cuda_attn_t* attn, float* out, const float* q,
+                     uint32_t n_seqs, uint32_t n_tokens, const int32_t* q_start, const int32_t* kv_len,
+                     const int32_t* pages, uint32_t pages_stride, const int32_t* prefix_pages, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* The next token of each of `rows` rows of logits (vocab values each,
+ * logits_stride floats apart, vocab up to 2^20) by a uniform number u[row] in
+ * [0, 1).  Candidates are the logits above -inf (NaN is none).  In the order
+ * of larger logit, then lower index: the first top_k (<= 0: all) stay; of
+ * these the shortest beginning that holds top_p of their probability at
+ * `temperature` (>= 1: all); of these those with at least min_p times the
+ * first one's probability.  The pick is the first in index order whose
+ * cumulative share of what stays exceeds u.  temperature <= 0 takes the
+ * first maximum (sampler.go:86-96).  Each of temperature, top_k, top_p and
+ * min_p is an array of rows values or NULL (1, all, 1, 0).  Weights are
+ * 64-bit integers, 2^42 for the largest, so ids do not depend on the order
+ * of any sum.  ids[row] is -1 in a row without candidates; prob (or NULL)
+ * receives the pick's share of what stayed. */
+int gi_cuda_sample_dev(int32_t* ids, float* prob, const float* logits, size_t logits_stride, uint32_t rows,
+                       uint32_t vocab, const float* u, const float* temperature, const int32_t* top_k,
+                       const float* top_p, const float* min_p, void* stream);
 
 #ifdef __cplusplus
 }
