@@ -173,7 +173,7 @@ int gi_cuda_attn_dev(const gi_cuda_kv_cache_t* cache, const gi_cuda_attn_t* attn
   if (int rc = attn_ref(c, attn, &a)) return rc;
   if (!out || !q || !kv_len || !pages || (a.prefix_len && !prefix_pages)) return fail(-4, "null device pointer");
   if (n_tokens > attn->max_tokens) return fail(-4, "more tokens than the call was described for");
-  if (n_seqs > (1u << 20)) return fail(-4, "too many sequences");
+  if (n_seqs > attn->max_tokens) return fail(-4, "more sequences than max_tokens");
   if (!q_start && n_tokens != n_seqs) return fail(-4, "without q_start a sequence has one token");
   if (!pages_stride || (uint64_t)pages_stride * c.page_size > INT32_MAX) return fail(-4, "pages_stride out of range");
   if (misaligned(out) || misaligned(q)) return fail(-4, "rows must be 16-byte aligned");

@@ -6,8 +6,30 @@
 // Sequence b has len = kv_len[b] cached positions in its own pages, the last
 // `new` of which are its tokens q_start[b] .. q_start[b+1] - 1 of this call.
 // Token j of them sees the whole prefix and its own positions below
-// len - new + j + 1; with nothing to see its row is 0.  Softmax statistics
-// and sums are float32.
+// len - new + j + 1; with nothing to see its row is 0.
+//
+// out = sum_t p_t v_t / sum_t p_t, p_t = 2^(s_t - m), s_t = log2(e) scale q.k_t,
+// in one pass over the positions with the running maximum m: a tile of
+// positions raises m, and what was summed before shrinks by 2^(m_old - m_new).
+//
+// The products run on the fp16 tensor cores (mma m16n8k16, float32 sums) and
+// keep float32's precision where it counts: the cache's values are halves
+// already (kvcache.cu), q and p are split into a half and the half of its
+// remainder (22 bits).  The 16 rows of an MMA are the high parts of 8 query
+// rows over their low parts, so a row's two sums end in one thread.
+// q rows are scaled by a power of two to just under 2^14 and p to at most 2^14, which
+// keeps the remainders in half's normal range.  An MMA chain is one
+// tile long; the running sum over tiles is a float32 FMA, because the tensor
+// cores cut their sums instead of rounding them and a chain of thousands of
+// positions would drift.
+//
+// Bound: single tokens read the cache once (HBM).  A unit of work is (sequence, kv
+// head, 8 * MT query rows of that head's group): it reads a position once for
+// all its rows.  The units' tiles form one line that is cut into equal runs, one per
+// CTA, so unequal lengths cost nothing and one long sequence fills the GPU; a
+// unit that is cut leaves parts (m, sum, row) that attn_merge_kernel joins in
+// order.  Each of a CTA's 4 warps takes every 4th tile of the run through a
+// cp.async ring of its own and meets the others only at the end of a unit.
 #include "common.cuh"
 #include "gemv.cuh"
 #include "serve.cuh"
@@ -15,87 +37,679 @@
 namespace gi {
 namespace {
 
-constexpr int kAttnThreads = 256;
+constexpr int kWarps = 4, kAttnThreads = 32 * kWarps;
+constexpr int kMergeThreads = 128;
+constexpr float kLog2e = 1.4426950408889634f;
 
-GI_DEVINL float cached(const KvCache& c, const uint8_t* plane, const __half* scales, size_t at) {
-  if (c.type == kTypeF16) return __half2float(reinterpret_cast<const __half*>(plane)[at]);
-  return __half2float(__hmul(__int2half_rn(reinterpret_cast<const int8_t*>(plane)[at]), scales[at >> 5]));
+GI_DEVINL float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
-// One (token, head) per block; a warp takes every 8th position and holds
-// head_dim / 32 dimensions per lane.
-template <int HD>
-__global__ void __launch_bounds__(kAttnThreads) attn_rows_kernel(KvCache c, Attn a) {
-  constexpr int E = HD / 32, W = kAttnThreads / 32;
-  __shared__ float so[W][HD], sm[W], sl[W];
-  const int token = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = h / (a.n_heads / c.n_kv_heads);
-  int b = 0, start = 0, end = 0;
-  for (; b < a.n_seqs; ++b) {
-    start = a.q_start ? a.q_start[b] : b;
-    end = a.q_start ? a.q_start[b + 1] : b + 1;
-    if (token >= start && token < end) break;
+// 16 bytes to shared memory, of which the first `bytes` (16 or 0) are read.
+GI_DEVINL void cp_async16_or_zero(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+GI_DEVINL void ldsm_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr));
+}
+
+// Four int8 codes as two half2 (exact): 0x6400 + (c + 128) is the half
+// 1152 + c.
+GI_DEVINL void codes_to_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  w ^= 0x80808080u;
+  lo = hsub2_u32(prmt(w, 0x64646464u, 0x4140), 0x64806480u);
+  hi = hsub2_u32(prmt(w, 0x64646464u, 0x4342), 0x64806480u);
+}
+
+// The positions and rows one launch covers: every sequence's own positions,
+// or the shared prefix as one sequence whose rows are all tokens.
+struct Pass {
+  const float* q;
+  float* out;   // rows of whole units: finished, or with ml not null the sums alone
+  float2* ml;   // [token][head] (m, sum) of whole units
+  float* parts;  // of units cut between CTAs, two slots per CTA
+  long long* line;  // [0] tiles per CTA, [1 + b] sequence b's first tile
+  const int32_t *q_start, *kv_len, *pages;
+  int pages_stride, n_seqs, n_tokens, n_heads;
+  int prefix;  // > 0: the prefix pass, of that many positions; n_seqs still counts the sequences
+  float scale;
+};
+
+struct Seq {
+  int start, fresh, len;  // first token, new tokens, positions
+};
+
+__host__ __device__ constexpr int pow2_up(int n) { return n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512; }
+
+GI_DEVINL Seq seq_of(const Pass& p, int b, int page_shift) {
+  Seq s;
+  const int first = p.prefix ? 0 : b, last = p.prefix ? p.n_seqs : b + 1;
+  s.start = max(0, min(p.q_start ? p.q_start[first] : first, p.n_tokens));
+  s.fresh = max(s.start, min(p.q_start ? p.q_start[last] : last, p.n_tokens)) - s.start;
+  s.len = p.prefix ? p.prefix : max(0, min(p.kv_len[b], p.pages_stride << page_shift));
+  return s;
+}
+
+// Positions of the sequence that new token j sees.
+GI_DEVINL int seen_by(const Pass& p, const Seq& s, int j) {
+  return p.prefix ? s.len : max(0, min(s.len, s.len - s.fresh + j + 1));
+}
+
+// HD head dim, MT groups of 8 query rows per unit, TT positions per tile.
+template <int HD, int TYPE, int MT, int TT>
+struct Tile {
+  static constexpr int kRows = 8 * MT;
+  static constexpr int kElem = TYPE == kTypeF16 ? 2 : 1;
+  static constexpr int kPitch = pow2_up(HD * kElem);      // bytes of a position's row in shared memory
+  static constexpr int kChunks = HD * kElem / 16;         // 16-byte chunks of a row
+  static constexpr int kScaleBytes = TYPE == kTypeF16 ? 0 : HD / 16;  // a position's scales
+  static constexpr int kPlane = TT * kPitch, kScales = TT * kScaleBytes;
+  static constexpr int kStage = 2 * (kPlane + kScales);
+  static constexpr int kQ = MT * (HD / 16) * 512;
+  static constexpr int kMerge = kWarps * kRows * HD * 4;
+  static constexpr int kRing = kWarps * 2 * kStage > kMerge ? kWarps * 2 * kStage : kMerge;
+  static constexpr int kSmem = kRing + kQ + kWarps * kRows * 8 + kRows * 4;
+  static constexpr int kPart = kRows * (HD + 2);  // floats of a part
+
+  // Chunk of row r that holds logical chunk c.  The reads of one instruction
+  // touch rows 0, 1, 4, 5, 8, 9, 12, 13 (K) or 0, 4, 8, 12 (V codes); the
+  // exclusive-or puts them in different banks.
+  GI_DEVINL static int chunk(int r, int c) {
+    if (TYPE == kTypeF16) return c ^ (((r & 1) << 2) | ((r >> 2) & 3));
+    if (HD == 64) return c ^ (((r >> 2) & 1) << 1);
+    return c ^ ((((r ^ (r >> 3)) & 1) | (((r >> 2) & 1) << 1)) << 1);
   }
-  if (b == a.n_seqs) return;  // behind the last sequence
-  const int own = max(0, min(a.kv_len[b], a.pages_stride * c.page_size));
-  const int seen = max(0, min(own, own - (end - start) + (token - start) + 1));
-  const size_t row = ((size_t)token * a.n_heads + h) * HD;
-  float q[E], o[E], m = -INFINITY, l = 0.f;
+};
+
+// Sequence tiles and units: rt row tiles per kv head, tl tiles per unit.
+struct Span {
+  int rt, tl;
+  long long tiles;
+};
+GI_DEVINL Span span_of(const Seq& s, int group, int kv_heads, int rows, int tt) {
+  Span n;
+  n.rt = (int)(((long long)s.fresh * group + rows - 1) / rows);
+  n.tl = max(1, (s.len + tt - 1) / tt);
+  n.tiles = (long long)n.rt * n.tl * kv_heads;
+  return n;
+}
+
+template <int HD, int TYPE, int MT, int TT, int MINB>
+__global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache c, Pass p) {
+  using T = Tile<HD, TYPE, MT, TT>;
+  constexpr int NT = TT / 8, NG = TT / 16, NB = HD / 32;
+  extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ long long s_scan[kWarps + 1], s_first;
+  __shared__ int s_seq;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int group = p.n_heads / c.n_kv_heads;
+  const int n_seqs = p.prefix ? 1 : p.n_seqs;
+
+  // ---- this CTA's run of the line of tiles ----
+  const int per = (n_seqs + kAttnThreads - 1) / kAttnThreads;
+  const int b0 = min(tid * per, n_seqs), b1 = min(b0 + per, n_seqs);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b)
+    mine += span_of(seq_of(p, b, c.page_shift), group, c.n_kv_heads, T::kRows, TT).tiles;
+  long long incl = mine;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = a.q[row + lane + 32 * e] * a.scale;
-    o[e] = 0.f;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
   }
-  for (int t = warp; t < a.prefix_len + seen; t += W) {
-    const int p = t < a.prefix_len ? t : t - a.prefix_len;
-    const int page = t < a.prefix_len ? a.prefix_pages[p >> c.page_shift]
-                                      : a.pages[(size_t)b * a.pages_stride + (p >> c.page_shift)];
-    if (page < 0 || page >= c.n_pages) continue;
-    const size_t at =
-        (((size_t)page * c.n_kv_heads + g) << c.page_shift | (p & (c.page_size - 1))) * HD + lane;
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(q[e], cached(c, c.k, c.ks, at + 32 * e), s);
-    s = warp_sum(s);
-    const float mn = fmaxf(m, s), f = m == -INFINITY ? 0.f : expf(m - mn), w = expf(s - mn);
-    l = l * f + w;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * f + w * cached(c, c.v, c.vs, at + 32 * e);
-    m = mn;
+  if (lane == 31) s_scan[warp] = incl;
+  __syncthreads();
+  long long before = incl - mine, total = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += s_scan[w];
+    total += s_scan[w];
   }
-#pragma unroll
-  for (int e = 0; e < E; ++e) so[warp][lane + 32 * e] = o[e];
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
+  // at least one tile for every warp
+  const long long chunk = max((total + gridDim.x - 1) / (long long)gridDim.x, (long long)kWarps);
+  long long pos = (long long)blockIdx.x * chunk;
+  const long long end = min(total, pos + chunk);
+  if (blockIdx.x == 0) {
+    if (tid == 0) p.line[0] = chunk;
+    long long at = before;
+    for (int b = b0; b < b1; ++b) {
+      p.line[1 + b] = at;
+      at += span_of(seq_of(p, b, c.page_shift), group, c.n_kv_heads, T::kRows, TT).tiles;
+    }
+  }
+  if (pos >= end) return;
+  if (pos >= before && pos < before + mine) {
+    long long at = before;
+    int b = b0;
+    for (;; ++b) {
+      const long long n = span_of(seq_of(p, b, c.page_shift), group, c.n_kv_heads, T::kRows, TT).tiles;
+      if (pos < at + n) break;
+      at += n;
+    }
+    s_seq = b;
+    s_first = at;
   }
   __syncthreads();
-  float M = -INFINITY, L = 0.f;
-  for (int w = 0; w < W; ++w) M = fmaxf(M, sm[w]);
-  for (int w = 0; w < W; ++w) L += sm[w] == -INFINITY ? 0.f : sl[w] * expf(sm[w] - M);
-  for (int d = threadIdx.x; d < HD; d += kAttnThreads) {
-    float x = 0.f;
-    for (int w = 0; w < W; ++w) x += sm[w] == -INFINITY ? 0.f : so[w][d] * expf(sm[w] - M);
-    a.out[row + d] = L > 0.f ? x / L : 0.f;
+  int b = s_seq;
+  long long first = s_first;
+
+  uint8_t* ring = sm + warp * 2 * T::kStage;
+  uint8_t* sq = sm + T::kRing;
+  float2* s_ml = reinterpret_cast<float2*>(sq + T::kQ);           // [warp][row]
+  float* s_fac = reinterpret_cast<float*>(s_ml + kWarps * T::kRows);  // [row]
+  const uint32_t ring_u = smem_u32(ring), sq_u = smem_u32(sq);
+
+  while (pos < end) {
+    Seq s = seq_of(p, b, c.page_shift);
+    Span n = span_of(s, group, c.n_kv_heads, T::kRows, TT);
+    while (pos >= first + n.tiles) {
+      first += n.tiles;
+      s = seq_of(p, ++b, c.page_shift);
+      n = span_of(s, group, c.n_kv_heads, T::kRows, TT);
+    }
+    const long long rel = pos - first;
+    const int unit = (int)(rel / n.tl), tile0 = (int)(rel - (long long)unit * n.tl);
+    const int h = unit / n.rt, row0 = (unit - h * n.rt) * T::kRows;
+    const int count = (int)min(end - pos, (long long)(n.tl - tile0));
+    const bool whole = count == n.tl;
+    pos += count;
+    const int n_rows = min(T::kRows, s.fresh * group - row0);
+    const int seen_first = seen_by(p, s, row0 / group), seen_last = seen_by(p, s, (row0 + n_rows - 1) / group);
+    const int tile_end = min(tile0 + count, (seen_last + TT - 1) / TT);
+    const int32_t* pages = p.pages + (p.prefix ? 0 : (size_t)b * p.pages_stride);
+
+    // Copies a tile into stage `st`; returns a bit per 16 positions whose page is not in the cache.
+    auto issue = [&](int tile, int st) {
+      uint32_t bad = 0;
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) {
+        const int p0 = tile * TT + gr * 16;
+        const int page = p0 < s.len ? __ldg(pages + (p0 >> c.page_shift)) : -1;
+        const bool ok = (unsigned)page < (unsigned)c.n_pages;
+        if (!ok) bad |= 1u << gr;
+        const size_t at =
+            ((size_t)(ok ? page : 0) * c.n_kv_heads + h << c.page_shift) + (ok ? p0 & (c.page_size - 1) : 0);
+        const uint32_t dst = ring_u + st * T::kStage;
+        const int left = ok ? s.len - p0 : 0;  // positions of the 16 that exist
+#pragma unroll
+        for (int i = lane; i < 16 * T::kChunks; i += 32) {
+          const int r = i / T::kChunks, ch = i - r * T::kChunks;
+          const uint32_t d = dst + (gr * 16 + r) * T::kPitch + T::chunk(r, ch) * 16;
+          const size_t src = at * HD * T::kElem + (size_t)i * 16;
+          const int bytes = r < left ? 16 : 0;
+          cp_async16_or_zero(d, c.k + src, bytes);
+          cp_async16_or_zero(d + T::kPlane, c.v + src, bytes);
+        }
+        if (TYPE == kTypeQ8_0) {
+          const uint32_t ds = dst + 2 * T::kPlane + gr * 16 * T::kScaleBytes;
+          for (int i = lane; i < T::kScaleBytes; i += 32) {
+            const size_t src = at * T::kScaleBytes + (size_t)i * 16;
+            const int bytes = i * 16 < left * T::kScaleBytes ? 16 : 0;
+            cp_async16_or_zero(ds + i * 16, reinterpret_cast<const uint8_t*>(c.ks) + src, bytes);
+            cp_async16_or_zero(ds + T::kScales + i * 16, reinterpret_cast<const uint8_t*>(c.vs) + src, bytes);
+          }
+        }
+      }
+      return bad;
+    };
+
+    int tile = tile0 + warp;
+    uint32_t bad = 0, bad_next = 0;
+    if (tile < tile_end) bad_next = issue(tile, 0);
+    cp_async_commit();
+
+    // ---- the unit's queries as MMA operands: a power of two under 2^14 per row, high and low halves ----
+    for (int r = warp; r < T::kRows; r += kWarps) {
+      const int row = row0 + r;
+      const bool real = r < n_rows;
+      const float* q = p.q + ((size_t)(s.start + (real ? row / group : 0)) * p.n_heads + (size_t)h * group +
+                              (real ? row % group : 0)) * HD;
+      float2 x[(HD / 2 + 31) / 32];
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < (HD / 2 + 31) / 32; ++i) {
+        const int d2 = lane + 32 * i;
+        x[i] = real && d2 < HD / 2 ? reinterpret_cast<const float2*>(q)[d2] : make_float2(0.f, 0.f);
+        m = fmaxf(m, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
+      }
+      m = warp_max(m);
+      const int ex = (int)(__float_as_uint(m) >> 23) - 127;  // m in [2^ex, 2^(ex + 1))
+      const int sh = m > 0.f ? min(13 - ex, 126) : 0;
+      const float up = exp2i(sh);
+      if (lane == 0) s_fac[r] = p.scale * kLog2e * exp2i(-sh);
+#pragma unroll
+      for (int i = 0; i < (HD / 2 + 31) / 32; ++i) {
+        const int d = 2 * (lane + 32 * i);
+        if (d >= HD) break;
+        // dimension d is byte d % 8 of quad d % 32 / 8's part of block d / 32
+        const int ks = (d >> 5) * 2 + ((d >> 2) & 1), reg = (d & 2);
+        const uint32_t hi = pack_h2(x[i].x * up, x[i].y * up);
+        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        const uint32_t lo = pack_h2(x[i].x * up - back.x, x[i].y * up - back.y);
+        uint32_t* w = reinterpret_cast<uint32_t*>(
+            sq + (((r >> 3) * (HD / 16) + ks) * 32 + (r & 7) * 4 + ((d >> 3) & 3)) * 16);
+        w[reg] = hi;
+        w[reg + 1] = lo;
+      }
+    }
+    __syncthreads();
+
+    float o[MT][HD / 8][2], m[MT], l[MT], fac[MT];
+    int seen[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int r = mt * 8 + g;
+      m[mt] = -INFINITY;
+      l[mt] = 0.f;
+      fac[mt] = s_fac[r];
+      seen[mt] = seen_by(p, s, (row0 + min(r, n_rows - 1)) / group);
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) o[mt][i][0] = o[mt][i][1] = 0.f;
+    }
+
+    for (int st = 0; tile < tile_end; tile += kWarps, st ^= 1) {
+      bad = bad_next;
+      if (tile + kWarps < tile_end) bad_next = issue(tile + kWarps, st ^ 1);
+      cp_async_commit();
+      cp_async_wait<1>();
+      __syncwarp();
+      const uint32_t ku = ring_u + st * T::kStage, vu = ku + T::kPlane, ksu = vu + T::kPlane, vsu = ksu + T::kScales;
+      const int p0 = tile * TT;
+      if (TYPE == kTypeQ8_0 && p0 + TT > s.len) {  // scales of positions that do not exist may hold anything
+        for (int i = lane; i < TT * (HD / 32); i += 32)
+          if (p0 + i / (HD / 32) >= s.len)
+            *reinterpret_cast<__half*>(ring + st * T::kStage + 2 * T::kPlane + T::kScales + 2 * i) = __half(0.f);
+        __syncwarp();
+      }
+
+      // S = q K^T: column g of MMA nt is position 16 (nt / 2) + 4 (g / 2) + g % 2 + 2 (nt % 2)
+      float sc[MT][NT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[mt][nt][i] = 0.f;
+#pragma unroll
+      for (int blk = 0; blk < NB; ++blk) {
+        uint4 a[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) a[mt][k] = lds128(sq_u + ((mt * (HD / 16) + 2 * blk + k) * 32 + lane) * 16);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const int r = 4 * (g >> 1) + (g & 1) + 2 * (nt & 1), row = 16 * (nt >> 1) + r;
+          uint32_t kb[4];
+          if (TYPE == kTypeF16) {
+            const uint4 w = lds128(ku + row * T::kPitch + T::chunk(r, 4 * blk + t) * 16);
+            kb[0] = w.x, kb[1] = w.y, kb[2] = w.z, kb[3] = w.w;
+          } else {
+            const uint64_t w = lds64(ku + row * T::kPitch + T::chunk(r, 2 * blk + (t >> 1)) * 16 + (t & 1) * 8);
+            const uint32_t d = lds16(ksu + row * T::kScaleBytes + 2 * blk), d2 = d | (d << 16);
+            codes_to_h2((uint32_t)w, kb[0], kb[1]);
+            codes_to_h2((uint32_t)(w >> 32), kb[2], kb[3]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) kb[i] = hmul2_u32(kb[i], d2);
+          }
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma_16816(sc[mt][nt], a[mt][0].x, a[mt][0].y, a[mt][0].z, a[mt][0].w, kb[0], kb[1]);
+            mma_16816(sc[mt][nt], a[mt][1].x, a[mt][1].y, a[mt][1].z, a[mt][1].w, kb[2], kb[3]);
+          }
+        }
+      }
+
+      // softmax: this thread's positions of row g are 16 (nt / 2) + 4 t + 2 (nt % 2) + {0, 1}
+      uint32_t pf[MT][NG][4];
+      float alpha[MT];
+      const bool masked = p0 + TT > seen_first || bad;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float x = (sc[mt][nt][i] + sc[mt][nt][i + 2]) * fac[mt];
+            if (masked) {
+              const int at = p0 + 16 * (nt >> 1) + 4 * t + 2 * (nt & 1) + i;
+              if (at >= seen[mt] || ((bad >> (nt >> 1)) & 1)) x = -INFINITY;
+            }
+            sc[mt][nt][i] = x;
+            top = fmaxf(top, x);
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float mn = fmaxf(m[mt], top), base = mn == -INFINITY ? 0.f : mn;
+        alpha[mt] = exp2_approx(m[mt] - base);
+        m[mt] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const float x = exp2_approx(sc[mt][nt][0] - base) * 16384.f, y = exp2_approx(sc[mt][nt][1] - base) * 16384.f;
+          sum += x + y;
+          const uint32_t hi = pack_h2(x, y);
+          const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+          pf[mt][nt >> 1][2 * (nt & 1)] = hi;
+          pf[mt][nt >> 1][2 * (nt & 1) + 1] = pack_h2(x - back.x, y - back.y);
+        }
+        l[mt] = l[mt] * alpha[mt] + sum;
+      }
+
+      // O += P V
+#pragma unroll
+      for (int blk = 0; blk < NB; ++blk) {
+        float acc[MT][4][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[mt][j][i] = 0.f;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          uint32_t vb[4][2];
+          if (TYPE == kTypeF16) {  // MMA j: dimensions 32 blk + 8 j + (0 .. 7)
+            const int i8 = lane & 7, mat = lane >> 3;
+            const int r = 4 * (i8 >> 1) + (i8 & 1) + 2 * (mat & 1), row = 16 * gr + r;
+#pragma unroll
+            for (int j = 0; j < 4; j += 2)
+              ldsm_x4_trans(vu + row * T::kPitch + T::chunk(r, 4 * blk + j + (mat >> 1)) * 16, vb[j][0], vb[j][1],
+                            vb[j + 1][0], vb[j + 1][1]);
+          } else {  // MMA j: dimensions 32 blk + 4 (0 .. 7) + j
+            uint32_t w[4], d[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = 4 * t + i, row = 16 * gr + r;
+              w[i] = lds32(vu + row * T::kPitch + T::chunk(r, 2 * blk + (g >> 2)) * 16 + (g & 3) * 4);
+              d[i] = lds16(vsu + row * T::kScaleBytes + 2 * blk);
+            }
+            const uint32_t d01 = d[0] | (d[1] << 16), d23 = d[2] | (d[3] << 16);
+            uint32_t x[4], y[4];
+            codes_to_h2(prmt(w[0], w[1], 0x5140), x[0], x[1]);  // dimensions 0, 1 of positions 0, 1
+            codes_to_h2(prmt(w[0], w[1], 0x7362), x[2], x[3]);
+            codes_to_h2(prmt(w[2], w[3], 0x5140), y[0], y[1]);
+            codes_to_h2(prmt(w[2], w[3], 0x7362), y[2], y[3]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              vb[j][0] = hmul2_u32(x[j], d01);
+              vb[j][1] = hmul2_u32(y[j], d23);
+            }
+          }
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              mma_16816(acc[mt][j], pf[mt][gr][0], pf[mt][gr][1], pf[mt][gr][2], pf[mt][gr][3], vb[j][0], vb[j][1]);
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              o[mt][4 * blk + j][i] = fmaf(o[mt][4 * blk + j][i], alpha[mt], acc[mt][j][i] + acc[mt][j][i + 2]);
+      }
+      __syncwarp();
+    }
+    cp_async_wait<0>();
+
+    // ---- the four warps' sums joined ----
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      l[mt] += __shfl_xor_sync(0xffffffffu, l[mt], 1);
+      l[mt] += __shfl_xor_sync(0xffffffffu, l[mt], 2);
+      if (t == 0) s_ml[warp * T::kRows + mt * 8 + g] = make_float2(m[mt], l[mt]);
+    }
+    __syncthreads();  // also: every ring is free
+    float* s_o = reinterpret_cast<float*>(sm) + (size_t)warp * T::kRows * HD;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int r = mt * 8 + g;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w * T::kRows + r].x);
+      const float f = top == -INFINITY ? 0.f : exp2_approx(m[mt] - top);
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) {
+        const int blk = i >> 2, j = i & 3;
+        if (TYPE == kTypeF16) {
+          *reinterpret_cast<float2*>(s_o + r * HD + 8 * i + 2 * t) = make_float2(o[mt][i][0] * f, o[mt][i][1] * f);
+        } else {
+          s_o[r * HD + 32 * blk + 8 * t + j] = o[mt][i][0] * f;
+          s_o[r * HD + 32 * blk + 8 * t + 4 + j] = o[mt][i][1] * f;
+        }
+      }
+    }
+    __syncthreads();
+    float* part = p.parts + (size_t)(2 * blockIdx.x + (tile0 > 0 ? 0 : 1)) * T::kPart;
+    for (int i = tid; i < n_rows * (HD / 4); i += kAttnThreads) {
+      const int r = i / (HD / 4), d = (i - r * (HD / 4)) * 4;
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w * T::kRows + r].x);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 e = s_ml[w * T::kRows + r];
+        sum += top == -INFINITY ? 0.f : e.y * exp2_approx(e.x - top);
+        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm) +
+                                                          ((size_t)w * T::kRows + r) * HD + d);
+        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+      }
+      if (!whole) {
+        *reinterpret_cast<float4*>(part + r * HD + d) = x;
+        if (d == 0) *reinterpret_cast<float2*>(part + T::kRows * HD + 2 * r) = make_float2(top, sum);
+        continue;
+      }
+      const int row = row0 + r;
+      const size_t at = (size_t)(s.start + row / group) * p.n_heads + (size_t)h * group + row % group;
+      if (p.ml) {
+        if (d == 0) p.ml[at] = make_float2(top, sum);
+      } else {
+        const float f = sum > 0.f ? 1.f / sum : 0.f;
+        x.x *= f, x.y *= f, x.z *= f, x.w *= f;
+      }
+      *reinterpret_cast<float4*>(p.out + at * HD + d) = x;
+    }
+    __syncthreads();
   }
+}
+
+// A row's sources in one pass: the whole unit's sums, or the parts of the CTAs [i0, i1] that its unit was cut into.
+struct Rows {
+  int rows, tt, part;  // of the pass's tiles
+};
+
+GI_DEVINL void join(float& top, float& sum, float4& x, float m, float l, float4 y) {
+  if (m == -INFINITY) return;
+  const float mn = fmaxf(top, m), a = exp2_approx(top - mn), f = exp2_approx(m - mn);
+  x.x = x.x * a + y.x * f, x.y = x.y * a + y.y * f, x.z = x.z * a + y.z * f, x.w = x.w * a + y.w * f;
+  sum = sum * a + l * f;
+  top = mn;
+}
+
+// Joins row (token, head) of the passes' parts, in the order of the
+// positions: the prefix, then the sequence's own.  One CTA per (token, kv head).
+__global__ void __launch_bounds__(kMergeThreads) attn_merge_kernel(KvCache c, Pass own, Rows ro, Pass pre, Rows rp,
+                                                                   float* __restrict__ out) {
+  __shared__ int s_b;
+  const int token = blockIdx.x, h = blockIdx.y, group = own.n_heads / c.n_kv_heads, hd = c.head_dim;
+  if (threadIdx.x == 0) {
+    int b = token < own.n_seqs ? token : -1;
+    if (own.q_start) {  // the last sequence that starts at or before the token and has it
+      int lo = 0, hi = own.n_seqs;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (own.q_start[mid] <= token) lo = mid;
+        else hi = mid;
+      }
+      b = own.q_start[lo] <= token && token < own.q_start[lo + 1] ? lo : -1;
+    }
+    s_b = b;
+  }
+  __syncthreads();
+  const int b = s_b;
+  if (b < 0) return;
+  for (int i = threadIdx.x; i < group * (hd / 4); i += kMergeThreads) {
+    const int hg = i / (hd / 4), d = (i - hg * (hd / 4)) * 4;
+    const size_t at = (size_t)token * own.n_heads + (size_t)h * group + hg;
+    float top = -INFINITY, sum = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    bool done = false;
+    for (int k = pre.prefix ? 0 : 1; k < 2; ++k) {
+      const Pass& p = k ? own : pre;
+      const Rows& w = k ? ro : rp;
+      const int sb = k ? b : 0;
+      const Seq s = seq_of(p, sb, c.page_shift);
+      const Span n = span_of(s, group, c.n_kv_heads, w.rows, w.tt);
+      const int row = (token - s.start) * group + hg;
+      const long long chunk = p.line[0];
+      const long long u0 = p.line[1 + sb] + ((long long)h * n.rt + row / w.rows) * n.tl, u1 = u0 + n.tl;
+      const long long i0 = u0 / chunk, i1 = (u1 - 1) / chunk;
+      if (i0 == i1) {
+        if (!p.ml) {  // finished by its CTA
+          done = true;
+          break;
+        }
+        const float2 e = p.ml[at];
+        join(top, sum, x, e.x, e.y, *reinterpret_cast<const float4*>(p.out + at * hd + d));
+        continue;
+      }
+      for (long long ci = i0; ci <= i1; ++ci) {
+        const float* part = p.parts + (size_t)(2 * ci + (ci * chunk > u0 ? 0 : 1)) * w.part;
+        const int r = row % w.rows;
+        const float2 e = *reinterpret_cast<const float2*>(part + w.rows * hd + 2 * r);
+        join(top, sum, x, e.x, e.y, *reinterpret_cast<const float4*>(part + r * hd + d));
+      }
+    }
+    if (done) continue;
+    const float f = sum > 0.f ? 1.f / sum : 0.f;
+    *reinterpret_cast<float4*>(out + at * hd + d) = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+  }
+}
+
+// ---- launch choices -----------------------------------------------------------
+typedef void (*TilesKernel)(KvCache, Pass);
+struct Choice {
+  TilesKernel fn;
+  int smem, per_sm;
+  Rows rows;
+};
+
+template <int HD, int TYPE, int MT, int TT, int MINB>
+Choice choice() {
+  using T = Tile<HD, TYPE, MT, TT>;
+  return {attn_tiles_kernel<HD, TYPE, MT, TT, MINB>, T::kSmem, MINB, {T::kRows, TT, T::kPart}};
+}
+
+// The kernel for units of `rows` query rows.
+template <int HD, int TYPE>
+Choice choose(int rows) {
+  constexpr int wide = TYPE == kTypeF16 || HD == 256 ? 16 : 32;
+  constexpr int few = HD == 256 ? (TYPE == kTypeF16 ? 1 : 2) : 3;
+  if (rows <= 8) return choice<HD, TYPE, 1, wide, few>();
+  if (rows <= 16 || HD == 256) return choice<HD, TYPE, 2, 16, HD == 256 ? 1 : 3>();
+  return choice<HD, TYPE, HD == 256 ? 2 : 4, 16, HD == 256 ? 1 : 2>();
+}
+
+Choice choose(const KvCache& c, int rows) {
+  const bool f16 = c.type == kTypeF16;
+  switch (c.head_dim) {
+    case 64: return f16 ? choose<64, kTypeF16>(rows) : choose<64, kTypeQ8_0>(rows);
+    case 96: return f16 ? choose<96, kTypeF16>(rows) : choose<96, kTypeQ8_0>(rows);
+    case 128: return f16 ? choose<128, kTypeF16>(rows) : choose<128, kTypeQ8_0>(rows);
+    default: return f16 ? choose<256, kTypeF16>(rows) : choose<256, kTypeQ8_0>(rows);
+  }
+}
+
+// The workspace: each pass's line and parts, and with a prefix the whole units' sums of both.
+struct Layout {
+  size_t line[2], parts[2], ml[2], sums, bytes;
+};
+Layout layout(const KvCache& c, const Attn& a, const Choice& own, const Choice& pre, int sm_count) {
+  Layout w = {};
+  auto take = [&](size_t bytes) {
+    const size_t at = w.bytes;
+    w.bytes += (bytes + 255) & ~(size_t)255;
+    return at;
+  };
+  const size_t rows = (size_t)a.max_tokens * a.n_heads;
+  w.line[0] = take(8 * ((size_t)a.max_tokens + 1));
+  w.parts[0] = take(sizeof(float) * 2 * own.per_sm * sm_count * own.rows.part);
+  if (a.prefix_len) {
+    w.line[1] = take(16);
+    w.parts[1] = take(sizeof(float) * 2 * pre.per_sm * sm_count * pre.rows.part);
+    for (size_t& m : w.ml) m = take(8 * rows);
+    w.sums = take(sizeof(float) * rows * c.head_dim);
+  }
+  return w;
+}
+
+int rows_of(long long tokens, int group) { return (int)(tokens * group < 1024 ? tokens * group : 1024); }
+
+template <int HD, int TYPE>
+int prepare() {
+  for (int rows : {8, 16, 32}) {
+    const Choice k = choose<HD, TYPE>(rows);
+    if (cudaFuncSetAttribute(k.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem) != cudaSuccess) return -5;
+  }
+  return 0;
 }
 
 }  // namespace
 
-int attn_prepare_device() { return 0; }
+int attn_prepare_device() {
+  return prepare<64, kTypeF16>() || prepare<64, kTypeQ8_0>() || prepare<96, kTypeF16>() || prepare<96, kTypeQ8_0>() ||
+                 prepare<128, kTypeF16>() || prepare<128, kTypeQ8_0>() || prepare<256, kTypeF16>() ||
+                 prepare<256, kTypeQ8_0>()
+             ? -5
+             : 0;
+}
 
 bool attn_head_dim_ok(int hd) { return hd == 64 || hd == 96 || hd == 128 || hd == 256; }
 
-size_t attn_workspace(const KvCache&, const Attn&, int) { return 0; }
+size_t attn_workspace(const KvCache& c, const Attn& a, int sm_count) {
+  const int group = a.n_heads / c.n_kv_heads;
+  return layout(c, a, choose(c, rows_of(a.max_q_len, group)), choose(c, rows_of(a.max_tokens, group)), sm_count).bytes;
+}
 
-cudaError_t attn_launch(const KvCache& c, const Attn& a, int, cudaStream_t s) {
-  const dim3 grid(a.n_tokens, a.n_heads);
-  switch (c.head_dim) {
-    case 64: attn_rows_kernel<64><<<grid, kAttnThreads, 0, s>>>(c, a); break;
-    case 96: attn_rows_kernel<96><<<grid, kAttnThreads, 0, s>>>(c, a); break;
-    case 128: attn_rows_kernel<128><<<grid, kAttnThreads, 0, s>>>(c, a); break;
-    default: attn_rows_kernel<256><<<grid, kAttnThreads, 0, s>>>(c, a); break;
+cudaError_t attn_launch(const KvCache& c, const Attn& a, int sm_count, cudaStream_t s) {
+  const int group = a.n_heads / c.n_kv_heads;
+  const Choice ko = choose(c, rows_of(a.max_q_len, group)), kp = choose(c, rows_of(a.max_tokens, group));
+  const Layout w = layout(c, a, ko, kp, sm_count);
+  uint8_t* ws = static_cast<uint8_t*>(a.ws);
+  Pass own = {};
+  own.q = a.q;
+  own.out = a.out;
+  own.ml = a.prefix_len ? reinterpret_cast<float2*>(ws + w.ml[0]) : nullptr;
+  own.parts = reinterpret_cast<float*>(ws + w.parts[0]);
+  own.line = reinterpret_cast<long long*>(ws + w.line[0]);
+  own.q_start = a.q_start;
+  own.kv_len = a.kv_len;
+  own.pages = a.pages;
+  own.pages_stride = a.pages_stride;
+  own.n_seqs = a.n_seqs;
+  own.n_tokens = a.n_tokens;
+  own.n_heads = a.n_heads;
+  own.scale = a.scale;
+  Pass pre = own;
+  pre.prefix = a.prefix_len;
+  if (a.prefix_len) {
+    pre.out = reinterpret_cast<float*>(ws + w.sums);
+    pre.ml = reinterpret_cast<float2*>(ws + w.ml[1]);
+    pre.parts = reinterpret_cast<float*>(ws + w.parts[1]);
+    pre.line = reinterpret_cast<long long*>(ws + w.line[1]);
+    pre.pages = a.prefix_pages;
+    kp.fn<<<kp.per_sm * sm_count, kAttnThreads, kp.smem, s>>>(c, pre);
   }
+  ko.fn<<<ko.per_sm * sm_count, kAttnThreads, ko.smem, s>>>(c, own);
+  attn_merge_kernel<<<dim3(a.n_tokens, c.n_kv_heads), kMergeThreads, 0, s>>>(c, own, ko.rows, pre, kp.rows, a.out);
   return cudaGetLastError();
 }
 

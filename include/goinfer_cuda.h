@@ -439,8 +439,8 @@ int gi_cuda_kv_read_dev(const gi_cuda_kv_cache_t* cache, float* k, float* v, con
                         void* stream);
 
 /* What an attention call's kernels and workspace are chosen by: n_heads query
- * heads (a multiple of the cache's n_kv_heads); at most max_tokens tokens in
- * a call and max_q_len of one sequence (choices follow max_q_len, results do not
+ * heads (a multiple of the cache's n_kv_heads); at most max_tokens tokens and
+ * as many sequences in a call, and max_q_len tokens of one sequence (choices follow max_q_len, results do not
  * depend on it); prefix_len positions that every sequence sees before its
  * own; scale on q.k. */
 typedef struct {

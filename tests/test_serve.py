@@ -99,6 +99,7 @@ def test_attention_refusals():
     refused(G.ERR_SHAPE, "null", a, 0, *args[1:], q_start_ptr=A)
     refused(G.ERR_SHAPE, "null", attention(c, prefix_len=20), *args, q_start_ptr=A)
     refused(G.ERR_SHAPE, "more tokens", a, A, A, 2, 9, A, A, 3, A, 1 << 30, q_start_ptr=A)
+    refused(G.ERR_SHAPE, "more sequences", a, A, A, 9, 8, A, A, 3, A, 1 << 30, q_start_ptr=A)
     refused(G.ERR_SHAPE, "without q_start", a, *args)
     refused(G.ERR_SHAPE, "pages_stride", a, A, A, 2, 8, A, A, 0, A, 1 << 30, q_start_ptr=A)
     refused(G.ERR_SHAPE, "pages_stride", a, A, A, 2, 8, A, A, 1 << 28, A, 1 << 30, q_start_ptr=A)

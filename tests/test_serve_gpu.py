@@ -197,7 +197,7 @@ class AttnCase:
         self.d = {"q": dev(self.q), "start": dev(self.start), "len": dev(self.lens, np.int32), "table": dev(self.table),
                   "prefix": dev(self.prefix_pages) if prefix else None}
         self.out = torch.full((self.tokens, heads, dim), 5.0, device="cuda:0")
-        self.att = G.Attention(self.gc, heads=heads, max_tokens=self.tokens, max_q_len=max(self.new), scale=self.scale,
+        self.att = G.Attention(self.gc, heads=heads, max_tokens=max(self.tokens, len(lens)), max_q_len=max(self.new), scale=self.scale,
                                prefix_len=prefix)
         self.ws = torch.full((max(self.att.workspace_bytes, 1),), 255, dtype=torch.uint8, device="cuda:0")
         self.stream = torch.cuda.Stream()
@@ -250,7 +250,7 @@ def test_attention_of_long_and_short_sequences(kind, lens):
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("heads,kv", [(2, 2), (8, 2), (7, 1)])
 @pytest.mark.parametrize("lens,new", [
-    ([5], [5]), ([64], [33]), ([100, 3, 20], [1, 3, 7]), ([40, 40, 0], [40, 1, 2]), ([3], [9]), ([150, 70], [97, 2])])
+    ([5], [5]), ([64], [33]), ([100, 3, 20], [1, 3, 7]), ([40, 40, 0], [40, 1, 2]), ([3], [9]), ([150, 70], [97, 2]), ([30, 50, 0, 9], [2, 0, 0, 1])])
 def test_attention_of_chunks(kind, dim, heads, kv, lens, new):
     """Causal inside the chunk; [3] with 9 new tokens: the first 6 rows see nothing."""
     AttnCase(sum(lens) + heads, kind, heads, kv, dim, 16, lens, new, pad=2).run()
