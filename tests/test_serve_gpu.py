@@ -375,6 +375,28 @@ def test_sample_mixed_rows(vocab):
               [0.95, 1.0, 0.5, 0.9, 0.5, 1.0, 0.0], [0.05, 0.0, 0.2, 0.01, 0.0, 0.0, 0.0])
 
 
+@pytest.mark.parametrize("rows,vocab", [(1, 1 << 20), (2, 400001), (40, 5000), (150, 3000), (300, 40), (70, 9001)])
+def test_sample_row_counts_and_large_vocabularies(rows, vocab):
+    """From a row spread over a cluster (and one too long for shared memory) to a CTA per row."""
+    rng = np.random.default_rng(rows)
+    x = (rng.normal(size=(rows, vocab)) * 2).astype(np.float32)
+    u = rng.random(rows, np.float32)
+    ks, ps = rng.choice([0, 3, 50, 600, 2000], rows), rng.choice([1.0, 0.97, 0.6], rows).astype(np.float32)
+    check_ids(x, u, t=rng.uniform(0.2, 2, rows).astype(np.float32), k=ks, p=ps, least=rng.choice([0.0, 0.01], rows))
+
+
+def test_sample_clustered_logits():
+    """Nearly all logits in one narrow band below a far outlier: the first bins separate nothing."""
+    rng = np.random.default_rng(6)
+    x = (rng.normal(size=(12, 20000)) * 1e-3).astype(np.float32)
+    x[:, 77] = rng.choice([1.0, 50.0], 12)
+    x[6:] = np.round(x[6:], 3)  # and hundreds of equal ones
+    x[:, 99] = -1e9
+    u = rng.random(12, np.float32)
+    check_ids(x, u, k=[1, 2, 600, 5000, 19999, 0] * 2)
+    check_ids(x, u, t=[5.0] * 12, k=[0, 10000, 19998] * 4, p=[0.3, 0.7, 0.999, 0.5] * 3)
+
+
 def test_sample_one_filter_at_a_time():
     rng = np.random.default_rng(1)
     x = (rng.normal(size=(64, 3001)) * 2).astype(np.float32)
