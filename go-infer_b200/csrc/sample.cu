@@ -28,9 +28,14 @@
 // shared memory.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "serve.cuh"
 
+#ifndef GI_F
+#define GI_F 3ll
+#endif
 namespace cg = cooperative_groups;
 
 namespace gi {
@@ -43,6 +48,7 @@ constexpr int kBins = 256;
 constexpr int kList = kThreads;      // candidates that are ranked directly
 constexpr int kMaxCluster = 8;
 constexpr int kMaxSlice = 48 * 1024;  // logits a CTA keeps in shared memory (192 KB)
+constexpr int kMaxSums = (1 << 20) / kMaxCluster / 128;  // sums of 128 neighbours of the longest slice
 constexpr int kFracBits = 42;         // a weight of 1 is 2^42
 constexpr u64 kOne = 1ull << kFracBits;
 
@@ -112,11 +118,11 @@ struct Item {
 // step between tells that all have read it.
 struct Shown {
   uint32_t count[2][kBins], lo[2][kBins], hi[2][kBins];  // candidates and weights of the bins
-  u64 first, sum[2];   // smallest place; sums
+  u64 first, sum;      // smallest place; weight that stays
   uint32_t least;      // smallest key of a candidate
   u64 range[2][2];     // smallest and largest place of a bin
   int n_items;
-  Item items[kList];
+  u64 items[kList];    // places
 };
 
 struct Shared {
@@ -127,7 +133,8 @@ struct Shared {
   double table[64];
   u64 found_before;
   u64 answer;
-  int found_bin, n_list;
+  int found_bin;
+  u64 sums[kMaxSums];
 };
 
 GI_DEVINL void add64(uint32_t* lo, uint32_t* hi, u64 w) {
@@ -165,7 +172,9 @@ GI_DEVINL u64 block_scan(u64 v, u64* part, u64* total) {
   return before;
 }
 
-__global__ void __launch_bounds__(kThreads) sample_kernel(Sample p, int slice, int resident) {
+// RES: the slice is in shared memory, else it is read from global memory each time.
+template <bool RES>
+__global__ void __launch_bounds__(kThreads) sample_kernel(Sample p, int slice) {
   extern __shared__ __align__(16) float row_sm[];
   __shared__ Shared s;
   cg::cluster_group cluster = cg::this_cluster();
@@ -173,37 +182,62 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(Sample p, int slice, i
   const int row = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int i0 = min(rank * slice, p.vocab), n = min(slice, p.vocab - i0);  // this CTA's logits
   const float* g = p.logits + (size_t)row * p.stride + i0;
-  const float* x = resident ? row_sm : g;
   const float t = p.temperature ? p.temperature[row] : 1.f;
   const int k = p.top_k ? p.top_k[row] : 0;
   const float top_p = p.top_p ? p.top_p[row] : 1.f;
   const float min_p = p.min_p ? p.min_p[row] : 0.f;
 
-  // ---- the slice into shared memory; first place, smallest key ----
-  u64 first = ~0ull;
-  uint32_t least = ~0u;
-  auto look = [&](float v, int i) {
-    const uint32_t key = key_of(v);
-    if (key == 0u) return;
-    first = min(first, place_of(key, (uint32_t)(i0 + i)));
-    least = min(least, key);
+  // f(what the cluster's CTA r shows, r) for every r, unrolled so that the remote loads are in flight together
+  auto each_rank = [&](auto f) {
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r)
+      if (r < ranks) f(static_cast<const Shown*>(cluster.map_shared_rank(&s.shown, r)), r);
   };
-  int done = 0;
-  if ((reinterpret_cast<uintptr_t>(g) & 15) == 0) {
-    for (int i = tid; i < n / 4; i += kThreads) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(g) + i);
-      if (resident) reinterpret_cast<float4*>(row_sm)[i] = v;
-      look(v.x, 4 * i), look(v.y, 4 * i + 1), look(v.z, 4 * i + 2), look(v.w, 4 * i + 3);
+  // Four logits from index i (a multiple of 4) of the slice on; -inf behind its end.
+  const bool aligned = (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+  auto from_global = [&](int i) {
+    if (aligned && i + 4 <= n) return __ldg(reinterpret_cast<const float4*>(g + i));
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = i + e < n ? __ldg(g + i + e) : -INFINITY;
+    return make_float4(v[0], v[1], v[2], v[3]);
+  };
+  auto four_at = [&](int i) { return RES ? *reinterpret_cast<const float4*>(row_sm + i) : from_global(i); };
+  // f(logit, its index) over the slice, four neighbours per thread and step.
+  const int steps = (n + 4 * kThreads - 1) / (4 * kThreads);
+  auto each = [&](auto f) {
+#pragma unroll 2
+    for (int r = 0; r < steps; ++r) {
+      const int i = 4 * (r * kThreads + tid);
+      if (i >= n) break;
+      const float4 v = four_at(i);
+      f(v.x, i0 + i), f(v.y, i0 + i + 1), f(v.z, i0 + i + 2), f(v.w, i0 + i + 3);
     }
-    done = n & ~3;
-  }
-  for (int i = done + tid; i < n; i += kThreads) {
-    const float v = __ldg(g + i);
-    if (resident) row_sm[i] = v;
-    look(v, i);
+  };
+
+  // ---- the slice into shared memory; first place, smallest candidate ----
+  float best = -INFINITY, low = INFINITY;
+  int best_i = -1;
+#pragma unroll 8
+  for (int r = 0; r < steps; ++r) {
+    const int i = 4 * (r * kThreads + tid);
+    if (i >= n) break;
+    const float4 q = from_global(i);
+    if (RES) *reinterpret_cast<float4*>(row_sm + i) = q;
+    const float v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (v[e] > best) {  // the first maximum stays
+        best = v[e];
+        best_i = i + e;
+      }
+      if (v[e] > -INFINITY) low = fminf(low, v[e]);
+    }
   }
   if (tid < 64) s.table[tid] = exp2((double)tid / 64.0);
   for (int i = tid; i < 2 * kBins; i += kThreads) s.shown.count[0][i] = s.shown.lo[0][i] = s.shown.hi[0][i] = 0;
+  u64 first = best_i < 0 ? ~0ull : place_of(key_of(best), (uint32_t)(i0 + best_i));
+  uint32_t least = best_i < 0 ? ~0u : key_of(low);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
@@ -213,24 +247,28 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(Sample p, int slice, i
     s.part[warp] = first;
     s.part2[warp] = least;
   }
-  if (tid == 0) s.shown.n_items = s.n_list = 0;
+  if (tid == 0) s.shown.n_items = 0;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kSampleWarps; ++w) {
-      first = min(first, s.part[w]);
-      least = min(least, (uint32_t)s.part2[w]);
+  if (warp == 0) {
+    first = s.part[lane & (kSampleWarps - 1)];
+    least = (uint32_t)s.part2[lane & (kSampleWarps - 1)];
+#pragma unroll
+    for (int o = kSampleWarps / 2; o > 0; o >>= 1) {
+      first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+      least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
     }
-    s.shown.first = first;
-    s.shown.least = least;
+    if (lane == 0) {
+      s.shown.first = first;
+      s.shown.least = least;
+    }
   }
   cluster.sync();
   first = ~0ull;
   least = ~0u;
-  for (int r = 0; r < ranks; ++r) {
-    const Shown* o = cluster.map_shared_rank(&s.shown, r);
+  each_rank([&](const Shown* o, int) {
     first = min(first, o->first);
     least = min(least, o->least);
-  }
+  });
   if (first == ~0ull || !(t > 0.f)) {
     if (rank == 0 && tid == 0) {
       p.ids[row] = first == ~0ull ? -1 : (int32_t)(uint32_t)first;
@@ -243,7 +281,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(Sample p, int slice, i
   const Weigh weigh = {top, 1.0 / (double)t, s.table};
   const float reach = 0.5f * top - 0.5f * float_of(least);  // halves: the difference may pass the largest float
   const float per_bin = top == INFINITY ? 0.f : reach > 0.f ? fminf(255.99f / reach, 3.0e38f) : 0.f;
-  auto bin_of = [&](float v) {  // linear in the logit
+  auto bin_of = [&](float v) {  // linear in the logit; kBins for what is no candidate
+    if (!(v > -INFINITY)) return kBins;
     if (top == INFINITY) return v == INFINITY ? 0 : kBins - 1;
     return min((int)((0.5f * top - 0.5f * v) * per_bin), kBins - 1);
   };
@@ -251,34 +290,34 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(Sample p, int slice, i
   int turn = 0;      // which of the twice-kept buffers
   u64 cut = ~0ull;   // survivors: places <= cut
 
-  // Bins of the row's survivors in [from, to]: by logit (shift < 0), or by
-  // (place - from) >> shift.  Leaves the whole row's bins in s.bin_*.
-  auto bins = [&](bool weights, u64 from, u64 to, int shift) {
+  // Bins of the row's survivors: by logit, or (BY_PLACE) those in [from, to] by (place - from) >> shift.
+  // Leaves the whole row's bins in s.bin_*.
+  auto bins = [&](auto by_place, bool weights, u64 from, u64 to, int shift) {
     Shown& o = s.shown;
-    for (int i = tid; i < n; i += kThreads) {
-      const float v = x[i];
-      const uint32_t key = key_of(v);
-      if (key == 0u) continue;
-      const u64 place = place_of(key, (uint32_t)(i0 + i));
-      if (place < from || place > to) continue;
-      const int b = shift < 0 ? bin_of(v) : (int)((place - from) >> shift);
+    each([&](float v, int i) {
+      int b = bin_of(v);
+      if (b == kBins) return;
+      if (decltype(by_place)::value || cut != ~0ull) {
+        const u64 place = place_of(key_of(v), (uint32_t)i);
+        if (place < from || place > to) return;
+        if (decltype(by_place)::value) b = (int)((place - from) >> shift);
+      }
       atomicAdd(&o.count[turn][b], 1u);
       if (weights) add64(&o.lo[turn][b], &o.hi[turn][b], weigh(v));
-    }
+    });
     cluster.sync();
     if (tid < kBins) {
       u64 c = 0, w = 0;
-      for (int r = 0; r < ranks; ++r) {
-        const Shown* q = cluster.map_shared_rank(&s.shown, r);
+      each_rank([&](const Shown* q, int) {
         c += q->count[turn][tid];
         if (weights) w += (u64)q->hi[turn][tid] << 32 | q->lo[turn][tid];
-      }
+      });
       s.bin_count[tid] = c;
       s.bin_weight[tid] = w;
     }
     turn ^= 1;
     // the buffers of the next step: their readers have passed this step's barrier
-    for (int i = tid; i < kBins; i += kThreads) o.count[turn][i] = o.lo[turn][i] = o.hi[turn][i] = 0;
+    if (tid < kBins) o.count[turn][tid] = o.lo[turn][tid] = o.hi[turn][tid] = 0;
     __syncthreads();
   };
   // The bin in which the running sum (of counts or weights) reaches `need`, and the sum before it.
@@ -291,49 +330,48 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(Sample p, int slice, i
       s.found_before = before;
     }
     __syncthreads();
+    return all;
   };
-  // The row's survivors that `take` accepts, at most kList, into s.list of every CTA.
+  // The row's survivors that `take` accepts, at most kList, into s.list of
+  // every CTA, each with its weight; empty items up to a multiple of 8.
   auto gather = [&](auto take) {
-    for (int i = tid; i < n; i += kThreads) {
-      const float v = x[i];
-      const uint32_t key = key_of(v);
-      if (key == 0u) continue;
-      const u64 place = place_of(key, (uint32_t)(i0 + i));
-      if (place > cut || !take(v, place)) continue;
-      s.shown.items[atomicAdd(&s.shown.n_items, 1)] = {place, weigh(v)};
-    }
+    each([&](float v, int i) {
+      if (!take(v, i)) return;
+      const u64 place = place_of(key_of(v), (uint32_t)i);
+      if (place <= cut) s.shown.items[atomicAdd(&s.shown.n_items, 1)] = place;
+    });
     cluster.sync();
-    int at = 0;
-    for (int r = 0; r < ranks; ++r) {
-      const Shown* q = cluster.map_shared_rank(&s.shown, r);
-      const int m = q->n_items;
-      if (tid < m) s.list[at + tid] = q->items[tid];
-      at += m;
-    }
-    if (tid == 0) s.n_list = at;
+    int at = 0, m[kMaxCluster];
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) m[r] = 0;
+    each_rank([&](const Shown* q, int r) { m[r] = q->n_items; });
+    u64 place = ~0ull;  // thread at + j takes item j of rank r
+    each_rank([&](const Shown* q, int r) {
+      if (tid >= at && tid < at + m[r]) place = q->items[tid - at];
+      at += m[r];
+    });
+    s.list[tid] = {place, place == ~0ull ? 0ull : weigh(float_of(~(uint32_t)(place >> 32)))};
     cluster.sync();  // the items are read: they may be written again
     if (tid == 0) s.shown.n_items = 0;
     __syncthreads();
+    return at;
   };
-  // cut = the place at which the running sum over the order reaches `need`; the level-0 bins are there.
+  // cut = the place at which the running sum over the order reaches `need`; the level-0 bins are there and located.
   auto descend = [&](bool weights, u64 need) {
-    locate(weights, need);
-    int b = s.found_bin;
+    int b = s.found_bin, m;
     u64 before = s.found_before;
     if (s.bin_count[b] <= kList) {
-      gather([&](float v, u64) { return bin_of(v) == b; });
+      m = gather([&](float v, int) { return bin_of(v) == b; });
     } else {
       // smallest and largest place of the bin's survivors
       u64 lo = ~0ull, hi = 0;
-      for (int i = tid; i < n; i += kThreads) {
-        const float v = x[i];
-        const uint32_t key = key_of(v);
-        if (key == 0u || bin_of(v) != b) continue;
-        const u64 place = place_of(key, (uint32_t)(i0 + i));
-        if (place > cut) continue;
+      each([&](float v, int i) {
+        if (bin_of(v) != b) return;
+        const u64 place = place_of(key_of(v), (uint32_t)i);
+        if (place > cut) return;
         lo = min(lo, place);
         hi = max(hi, place);
-      }
+      });
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
@@ -345,38 +383,48 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(Sample p, int slice, i
         s.part2[warp] = hi;
       }
       __syncthreads();
-      if (tid == 0) {
-        for (int w = 0; w < kSampleWarps; ++w) {
-          lo = min(lo, s.part[w]);
-          hi = max(hi, s.part2[w]);
+      if (warp == 0) {
+        lo = s.part[lane & (kSampleWarps - 1)];
+        hi = s.part2[lane & (kSampleWarps - 1)];
+#pragma unroll
+        for (int o = kSampleWarps / 2; o > 0; o >>= 1) {
+          lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+          hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
         }
-        s.shown.range[turn][0] = lo;
-        s.shown.range[turn][1] = hi;
+        if (lane == 0) {
+          s.shown.range[turn][0] = lo;
+          s.shown.range[turn][1] = hi;
+        }
       }
       cluster.sync();
-      for (int r = 0; r < ranks; ++r) {
-        const Shown* q = cluster.map_shared_rank(&s.shown, r);
+      each_rank([&](const Shown* q, int) {
         lo = min(lo, q->range[turn][0]);
         hi = max(hi, q->range[turn][1]);
-      }
-      for (;;) {  // each turn leaves at most 1/128 of the range
+      });
+      u64 left;
+      do {  // each turn leaves at most 1/128 of the range
         const int shift = max(0, 56 - __clzll((long long)(hi - lo)));  // (hi - lo) >> shift < 256
-        bins(weights, lo, hi, shift);
+        bins(std::true_type(), weights, lo, hi, shift);
         locate(weights, need - before);
         const int d = s.found_bin;
         before += s.found_before;
         lo += (u64)d << shift;
         hi = min(hi, lo + ((1ull << shift) - 1));
-        const u64 left = s.bin_count[d];
-        if (left <= kList) break;
-      }
-      gather([&](float, u64 place) { return place >= lo && place <= hi; });
+        left = s.bin_count[d];
+      } while (left > kList);
+      m = gather([&](float v, int i) {
+        const u64 place = place_of(key_of(v), (uint32_t)i);
+        return v > -INFINITY && place >= lo && place <= hi;
+      });
     }
-    if (tid < s.n_list) {
+    if (tid < m) {
       const Item me = s.list[tid];
       u64 sum = before;
-      for (int j = 0; j < s.n_list; ++j)
-        if (s.list[j].place < me.place) sum += weights ? s.list[j].weight : 1ull;
+#pragma unroll 8
+      for (int j = 0; j < m; ++j) {
+        const Item e = s.list[j];
+        if (e.place < me.place) sum += weights ? e.weight : 1ull;
+      }
       if (sum < need && need <= sum + (weights ? me.weight : 1ull)) s.answer = me.place;
     }
     __syncthreads();
@@ -395,38 +443,43 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(Sample p, int slice, i
   };
 
   if (k > 0 && k < p.vocab) {
-    bins(false, 0ull, ~0ull, -1);
-    const u64 all = block_sum(tid < kBins ? s.bin_count[tid] : 0ull, s.part);
+    bins(std::false_type(), false, 0ull, ~0ull, 0);
+    const u64 all = locate(false, (u64)k);
     if (all > (u64)k) {
-      locate(false, (u64)k);
       const int b = s.found_bin;
       if (s.found_before + s.bin_count[b] <= kList) {
         // ---- the first k are on one list: finish on it ----
-        gather([&](float v, u64) { return bin_of(v) <= b; });
-        const int m = s.n_list;
-        Item me = {~0ull, 0ull};
+        const int m = gather([&](float v, int) { return bin_of(v) <= b; });
+        const Item me = s.list[tid];
         u64 before = 0;
         int ahead = 0;
         if (tid < m) {
-          me = s.list[tid];
-          for (int j = 0; j < m; ++j)
-            if (s.list[j].place < me.place) {
-              before += s.list[j].weight;
+#pragma unroll 8
+          for (int j = 0; j < m; ++j) {
+            const Item e = s.list[j];
+            if (e.place < me.place) {
+              before += e.weight;
               ++ahead;
             }
+          }
         }
         bool stays = tid < m && ahead < k;
-        const u64 sum = block_sum(stays ? me.weight : 0ull, s.part);
-        if (top_p < 1.f) stays = stays && before < needed(sum);
+        if (top_p < 1.f) {
+          const u64 sum = block_sum(stays ? me.weight : 0ull, s.part);
+          stays = stays && before < needed(sum);
+        }
         stays = stays && me.weight >= floor_w;
         __syncthreads();
-        if (tid < m) s.list[tid].weight = stays ? me.weight : 0ull;
+        s.list[tid].weight = stays ? me.weight : 0ull;
         const u64 total = block_sum(stays ? me.weight : 0ull, s.part);  // its barriers order the list's writes too
         if (stays && rank == 0) {
           const u64 target = target_of(total);
           u64 run = 0;
-          for (int j = 0; j < m; ++j)
-            if ((uint32_t)s.list[j].place < (uint32_t)me.place) run += s.list[j].weight;
+#pragma unroll 8
+          for (int j = 0; j < m; ++j) {
+            const Item e = s.list[j];
+            if ((uint32_t)e.place < (uint32_t)me.place) run += e.weight;
+          }
           if (run <= target && target < run + me.weight) {
             p.ids[row] = (int32_t)(uint32_t)me.place;
             if (p.prob) p.prob[row] = (float)((double)me.weight / (double)total);
@@ -438,52 +491,75 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(Sample p, int slice, i
     }
   }
   if (top_p < 1.f) {
-    bins(true, 0ull, cut, -1);
+    bins(std::false_type(), true, 0ull, cut, 0);
     const u64 sum = block_sum(tid < kBins ? s.bin_weight[tid] : 0ull, s.part);
     const u64 need = needed(sum);
-    if (need < sum) descend(true, need);
+    if (need < sum) {
+      locate(true, need);
+      descend(true, need);
+    }
   }
 
-  // ---- the pick: a thread sums a run of the slice (an odd length: no two lanes in one bank) ----
-  const int run = ((n + kThreads - 1) / kThreads) | 1, a0 = min(tid * run, n), a1 = min(a0 + run, n);
-  auto stays_weight = [&](int i) {
-    const float v = x[i];
-    const uint32_t key = key_of(v);
-    if (key == 0u || place_of(key, (uint32_t)(i0 + i)) > cut) return 0ull;
+  // ---- the pick: sums of 128 neighbours each (a warp's step), the sums scanned in index order ----
+  auto stays_weight = [&](float v, int i) {
+    if (!(v > -INFINITY) || place_of(key_of(v), (uint32_t)i) > cut) return 0ull;
     const u64 w = weigh(v);
     return w >= floor_w ? w : 0ull;
   };
+  auto four_weights = [&](int i, u64 (&w)[4]) {
+    const float4 v = i < n ? four_at(i) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    w[0] = stays_weight(v.x, i0 + i), w[1] = stays_weight(v.y, i0 + i + 1);
+    w[2] = stays_weight(v.z, i0 + i + 2), w[3] = stays_weight(v.w, i0 + i + 3);
+  };
+  for (int r = 0; r < steps; ++r) {
+    u64 w[4];
+    four_weights(4 * (r * kThreads + tid), w);
+    const u64 sum = warp_sum64(w[0] + w[1] + w[2] + w[3]);
+    if (lane == 0) s.sums[r * kSampleWarps + warp] = sum;
+  }
+  __syncthreads();
+  const int per = (steps * kSampleWarps + kThreads - 1) / kThreads;  // sums per thread: 1, or a few of a long slice
   u64 mine = 0;
-  for (int i = a0; i < a1; ++i) mine += stays_weight(i);
+  for (int e = 0; e < per; ++e)
+    if (tid * per + e < steps * kSampleWarps) mine += s.sums[tid * per + e];
   u64 here;
   u64 before = block_scan(mine, s.part, &here);
-  if (tid == 0) s.shown.sum[0] = here;
+  if (tid == 0) s.shown.sum = here;
   cluster.sync();
   u64 total = 0, ahead = 0;
-  for (int r = 0; r < ranks; ++r) {
-    const u64 w = cluster.map_shared_rank(&s.shown, r)->sum[0];
+  each_rank([&](const Shown* q, int r) {
+    const u64 w = q->sum;
     if (r < rank) ahead += w;
     total += w;
-  }
+  });
   cluster.sync();
   const u64 target = target_of(total);
+  if (target < ahead || target >= ahead + here) return;  // in another CTA's slice
   before += ahead;
-  if (target < before || target >= before + mine) return;
-  for (int i = a0; i < a1; ++i) {
-    const u64 w = stays_weight(i);
-    if (target < before + w) {
-      p.ids[row] = i0 + i;
-      if (p.prob) p.prob[row] = (float)((double)w / (double)total);
-      return;
-    }
-    before += w;
+  if (target >= before && target < before + mine) {
+    int e = tid * per;
+    while (target >= before + s.sums[e]) before += s.sums[e++];
+    s.found_bin = e;
+    s.found_before = before;
   }
+  __syncthreads();
+  if (warp != 0) return;
+  const int i = 128 * s.found_bin + 4 * lane;
+  u64 w[4];
+  four_weights(i, w);
+  const u64 sum = w[0] + w[1] + w[2] + w[3];
+  u64 at = s.found_before + warp_scan64(sum, lane) - sum;
+  if (target < at || target >= at + sum) return;
+  int e = 0;
+  while (target >= at + w[e]) at += w[e++];
+  p.ids[row] = i0 + i + e;
+  if (p.prob) p.prob[row] = (float)((double)w[e] / (double)total);
 }
 
 }  // namespace
 
 int sample_prepare_device() {
-  return cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  return cudaFuncSetAttribute(sample_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               kMaxSlice * (int)sizeof(float)) == cudaSuccess
              ? 0
              : -5;
@@ -494,10 +570,10 @@ cudaError_t sample_launch(const Sample& p, int sm_count, cudaStream_t s) {
   // shared memory
   int ranks = 1;
   while (ranks < kMaxCluster && (p.vocab > ranks * kMaxSlice ||
-                                 (p.vocab > ranks * 1024 && (long long)p.rows * ranks * 2 <= 3ll * sm_count)))
+                                 (p.vocab > ranks * 1024 && (long long)p.rows * ranks * 2 <= GI_F * sm_count)))
     ranks *= 2;
   const int slice = ((p.vocab + ranks - 1) / ranks + 3) & ~3;
-  const int resident = slice <= kMaxSlice;
+  const bool resident = slice <= kMaxSlice;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ranks * (unsigned)p.rows);
   cfg.blockDim = dim3(kThreads);
@@ -509,7 +585,8 @@ cudaError_t sample_launch(const Sample& p, int sm_count, cudaStream_t s) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_kernel, p, slice, resident);
+  return resident ? cudaLaunchKernelEx(&cfg, sample_kernel<true>, p, slice)
+                  : cudaLaunchKernelEx(&cfg, sample_kernel<false>, p, slice);
 }
 
 }  // namespace gi
