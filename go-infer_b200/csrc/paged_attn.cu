@@ -66,6 +66,33 @@ GI_DEVINL void codes_to_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {
   hi = hsub2_u32(prmt(w, 0x64646464u, 0x4342), 0x64806480u);
 }
 
+// D = A(16x16 f16, row) * B(16x8 f16, col): the first of a chain.
+GI_DEVINL void mma_16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                               uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// The scales of one position's blocks 0 .. N - 1, two halves a register.
+template <int N>
+GI_DEVINL void load_scales(uint32_t addr, uint32_t (&w)[(N + 1) / 2]) {
+  if (N == 2) {
+    w[0] = lds32(addr);
+  } else if (N == 4) {
+    const uint64_t x = lds64(addr);
+    w[0] = (uint32_t)x, w[(N + 1) / 2 - 1] = (uint32_t)(x >> 32);
+  } else if (N == 8) {
+    const uint4 x = lds128(addr);
+    w[0] = x.x, w[1 % ((N + 1) / 2)] = x.y, w[2 % ((N + 1) / 2)] = x.z, w[3 % ((N + 1) / 2)] = x.w;
+  } else {  // 3: six bytes, even alignment
+    w[0] = lds16(addr) | (lds16(addr + 2) << 16);
+    w[(N + 1) / 2 - 1] = lds16(addr + 4);
+  }
+}
+
 // The positions and rows one launch covers: every sequence's own positions,
 // or the shared prefix as one sequence whose rows are all tokens.
 struct Pass {
@@ -100,8 +127,9 @@ GI_DEVINL int seen_by(const Pass& p, const Seq& s, int j) {
   return p.prefix ? s.len : max(0, min(s.len, s.len - s.fresh + j + 1));
 }
 
-// HD head dim, MT groups of 8 query rows per unit, TT positions per tile.
-template <int HD, int TYPE, int MT, int TT>
+// HD head dim, MT groups of 8 query rows per unit, TT positions per tile, NS
+// tiles in a warp's ring.
+template <int HD, int TYPE, int MT, int TT, int NS>
 struct Tile {
   static constexpr int kRows = 8 * MT;
   static constexpr int kElem = TYPE == kTypeF16 ? 2 : 1;
@@ -112,7 +140,7 @@ struct Tile {
   static constexpr int kStage = 2 * (kPlane + kScales);
   static constexpr int kQ = MT * (HD / 16) * 512;
   static constexpr int kMerge = kWarps * kRows * HD * 4;
-  static constexpr int kRing = kWarps * 2 * kStage > kMerge ? kWarps * 2 * kStage : kMerge;
+  static constexpr int kRing = kWarps * NS * kStage > kMerge ? kWarps * NS * kStage : kMerge;
   static constexpr int kSmem = kRing + kQ + kWarps * kRows * 8 + kRows * 4;
   static constexpr int kPart = kRows * (HD + 2);  // floats of a part
 
@@ -126,6 +154,11 @@ struct Tile {
   }
 };
 
+// a / b, which fits an int; a >= 0
+GI_DEVINL int quotient(long long a, int b) {
+  return a < (1ll << 32) ? (int)((uint32_t)a / (uint32_t)b) : (int)(a / b);
+}
+
 // Sequence tiles and units: rt row tiles per kv head, tl tiles per unit.
 struct Span {
   int rt, tl;
@@ -133,15 +166,15 @@ struct Span {
 };
 GI_DEVINL Span span_of(const Seq& s, int group, int kv_heads, int rows, int tt) {
   Span n;
-  n.rt = (int)(((long long)s.fresh * group + rows - 1) / rows);
+  n.rt = (s.fresh * group + rows - 1) / rows;  // rows: a power of two; n_tokens * n_heads fits an int
   n.tl = max(1, (s.len + tt - 1) / tt);
   n.tiles = (long long)n.rt * n.tl * kv_heads;
   return n;
 }
 
-template <int HD, int TYPE, int MT, int TT, int MINB>
+template <int HD, int TYPE, int MT, int TT, int NS, int MINB>
 __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache c, Pass p) {
-  using T = Tile<HD, TYPE, MT, TT>;
+  using T = Tile<HD, TYPE, MT, TT, NS>;
   constexpr int NT = TT / 8, NG = TT / 16, NB = HD / 32;
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ long long s_scan[kWarps + 1], s_first;
@@ -154,6 +187,8 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
   const int per = (n_seqs + kAttnThreads - 1) / kAttnThreads;
   const int b0 = min(tid * per, n_seqs), b1 = min(b0 + per, n_seqs);
   long long mine = 0;
+  griddep_wait();
+  griddep_launch_dependents();
   for (int b = b0; b < b1; ++b)
     mine += span_of(seq_of(p, b, c.page_shift), group, c.n_kv_heads, T::kRows, TT).tiles;
   long long incl = mine;
@@ -197,7 +232,7 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
   int b = s_seq;
   long long first = s_first;
 
-  uint8_t* ring = sm + warp * 2 * T::kStage;
+  uint8_t* ring = sm + warp * NS * T::kStage;
   uint8_t* sq = sm + T::kRing;
   float2* s_ml = reinterpret_cast<float2*>(sq + T::kQ);           // [warp][row]
   float* s_fac = reinterpret_cast<float*>(s_ml + kWarps * T::kRows);  // [row]
@@ -212,7 +247,7 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
       n = span_of(s, group, c.n_kv_heads, T::kRows, TT);
     }
     const long long rel = pos - first;
-    const int unit = (int)(rel / n.tl), tile0 = (int)(rel - (long long)unit * n.tl);
+    const int unit = quotient(rel, n.tl), tile0 = (int)(rel - (long long)unit * n.tl);
     const int h = unit / n.rt, row0 = (unit - h * n.rt) * T::kRows;
     const int count = (int)min(end - pos, (long long)(n.tl - tile0));
     const bool whole = count == n.tl;
@@ -258,11 +293,15 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
     };
 
     int tile = tile0 + warp;
-    uint32_t bad = 0, bad_next = 0;
-    if (tile < tile_end) bad_next = issue(tile, 0);
-    cp_async_commit();
+    uint32_t bad[NS];  // of the stage `st + i`
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) {
+      bad[i] = tile + i * kWarps < tile_end ? issue(tile + i * kWarps, i) : 0u;
+      cp_async_commit();
+    }
 
     // ---- the unit's queries as MMA operands: a power of two under 2^14 per row, high and low halves ----
+#pragma unroll 2
     for (int r = warp; r < T::kRows; r += kWarps) {
       const int row = row0 + r;
       const bool real = r < n_rows;
@@ -311,11 +350,14 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
       for (int i = 0; i < HD / 8; ++i) o[mt][i][0] = o[mt][i][1] = 0.f;
     }
 
-    for (int st = 0; tile < tile_end; tile += kWarps, st ^= 1) {
-      bad = bad_next;
-      if (tile + kWarps < tile_end) bad_next = issue(tile + kWarps, st ^ 1);
+    for (int st = 0; tile < tile_end; tile += kWarps, st = st + 1 == NS ? 0 : st + 1) {
+      const uint32_t bad_now = bad[0];
+#pragma unroll
+      for (int i = 0; i < NS - 2; ++i) bad[i] = bad[i + 1];
+      bad[NS - 2] = 0;
+      if (tile + (NS - 1) * kWarps < tile_end) bad[NS - 2] = issue(tile + (NS - 1) * kWarps, st == 0 ? NS - 1 : st - 1);
       cp_async_commit();
-      cp_async_wait<1>();
+      cp_async_wait<NS - 1>();
       __syncwarp();
       const uint32_t ku = ring_u + st * T::kStage, vu = ku + T::kPlane, ksu = vu + T::kPlane, vsu = ksu + T::kScales;
       const int p0 = tile * TT;
@@ -328,12 +370,12 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
 
       // S = q K^T: column g of MMA nt is position 16 (nt / 2) + 4 (g / 2) + g % 2 + 2 (nt % 2)
       float sc[MT][NT][4];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      uint32_t kd[NT][(NB + 1) / 2];
+      if (TYPE == kTypeQ8_0) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sc[mt][nt][i] = 0.f;
+          load_scales<NB>(ksu + (16 * (nt >> 1) + 4 * (g >> 1) + (g & 1) + 2 * (nt & 1)) * T::kScaleBytes, kd[nt]);
+      }
 #pragma unroll
       for (int blk = 0; blk < NB; ++blk) {
         uint4 a[MT][2];
@@ -350,7 +392,7 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
             kb[0] = w.x, kb[1] = w.y, kb[2] = w.z, kb[3] = w.w;
           } else {
             const uint64_t w = lds64(ku + row * T::kPitch + T::chunk(r, 2 * blk + (t >> 1)) * 16 + (t & 1) * 8);
-            const uint32_t d = lds16(ksu + row * T::kScaleBytes + 2 * blk), d2 = d | (d << 16);
+            const uint32_t d2 = prmt(kd[nt][blk >> 1], 0u, blk & 1 ? 0x3232 : 0x1010);
             codes_to_h2((uint32_t)w, kb[0], kb[1]);
             codes_to_h2((uint32_t)(w >> 32), kb[2], kb[3]);
 #pragma unroll
@@ -358,7 +400,8 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
           }
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            mma_16816(sc[mt][nt], a[mt][0].x, a[mt][0].y, a[mt][0].z, a[mt][0].w, kb[0], kb[1]);
+            if (blk == 0) mma_16816_first(sc[mt][nt], a[mt][0].x, a[mt][0].y, a[mt][0].z, a[mt][0].w, kb[0], kb[1]);
+            else mma_16816(sc[mt][nt], a[mt][0].x, a[mt][0].y, a[mt][0].z, a[mt][0].w, kb[0], kb[1]);
             mma_16816(sc[mt][nt], a[mt][1].x, a[mt][1].y, a[mt][1].z, a[mt][1].w, kb[2], kb[3]);
           }
         }
@@ -367,7 +410,7 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
       // softmax: this thread's positions of row g are 16 (nt / 2) + 4 t + 2 (nt % 2) + {0, 1}
       uint32_t pf[MT][NG][4];
       float alpha[MT];
-      const bool masked = p0 + TT > seen_first || bad;
+      const bool masked = p0 + TT > seen_first || bad_now;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         float top = -INFINITY;
@@ -378,7 +421,7 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
             float x = (sc[mt][nt][i] + sc[mt][nt][i + 2]) * fac[mt];
             if (masked) {
               const int at = p0 + 16 * (nt >> 1) + 4 * t + 2 * (nt & 1) + i;
-              if (at >= seen[mt] || ((bad >> (nt >> 1)) & 1)) x = -INFINITY;
+              if (at >= seen[mt] || ((bad_now >> (nt >> 1)) & 1)) x = -INFINITY;
             }
             sc[mt][nt][i] = x;
             top = fmaxf(top, x);
@@ -402,15 +445,16 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
       }
 
       // O += P V
+      uint32_t vd[NG][4][(NB + 1) / 2];
+      if (TYPE == kTypeQ8_0) {
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) load_scales<NB>(vsu + (16 * gr + 4 * t + i) * T::kScaleBytes, vd[gr][i]);
+      }
 #pragma unroll
       for (int blk = 0; blk < NB; ++blk) {
         float acc[MT][4][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[mt][j][i] = 0.f;
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) {
           uint32_t vb[4][2];
@@ -422,14 +466,15 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
               ldsm_x4_trans(vu + row * T::kPitch + T::chunk(r, 4 * blk + j + (mat >> 1)) * 16, vb[j][0], vb[j][1],
                             vb[j + 1][0], vb[j + 1][1]);
           } else {  // MMA j: dimensions 32 blk + 4 (0 .. 7) + j
-            uint32_t w[4], d[4];
+            uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int r = 4 * t + i, row = 16 * gr + r;
               w[i] = lds32(vu + row * T::kPitch + T::chunk(r, 2 * blk + (g >> 2)) * 16 + (g & 3) * 4);
-              d[i] = lds16(vsu + row * T::kScaleBytes + 2 * blk);
             }
-            const uint32_t d01 = d[0] | (d[1] << 16), d23 = d[2] | (d[3] << 16);
+            const uint32_t sel = blk & 1 ? 0x7632 : 0x5410;
+            const uint32_t d01 = prmt(vd[gr][0][blk >> 1], vd[gr][1][blk >> 1], sel);
+            const uint32_t d23 = prmt(vd[gr][2][blk >> 1], vd[gr][3][blk >> 1], sel);
             uint32_t x[4], y[4];
             codes_to_h2(prmt(w[0], w[1], 0x5140), x[0], x[1]);  // dimensions 0, 1 of positions 0, 1
             codes_to_h2(prmt(w[0], w[1], 0x7362), x[2], x[3]);
@@ -445,7 +490,10 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              mma_16816(acc[mt][j], pf[mt][gr][0], pf[mt][gr][1], pf[mt][gr][2], pf[mt][gr][3], vb[j][0], vb[j][1]);
+              if (gr == 0)
+                mma_16816_first(acc[mt][j], pf[mt][gr][0], pf[mt][gr][1], pf[mt][gr][2], pf[mt][gr][3], vb[j][0], vb[j][1]);
+              else
+                mma_16816(acc[mt][j], pf[mt][gr][0], pf[mt][gr][1], pf[mt][gr][2], pf[mt][gr][3], vb[j][0], vb[j][1]);
         }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -526,66 +574,102 @@ struct Rows {
   int rows, tt, part;  // of the pass's tiles
 };
 
-GI_DEVINL void join(float& top, float& sum, float4& x, float m, float l, float4 y) {
-  if (m == -INFINITY) return;
-  const float mn = fmaxf(top, m), a = exp2_approx(top - mn), f = exp2_approx(m - mn);
-  x.x = x.x * a + y.x * f, x.y = x.y * a + y.y * f, x.z = x.z * a + y.z * f, x.w = x.w * a + y.w * f;
-  sum = sum * a + l * f;
-  top = mn;
-}
-
 // Joins row (token, head) of the passes' parts, in the order of the
 // positions: the prefix, then the sequence's own.  One CTA per (token, kv head).
+// Parts come in groups of kAhead, whose loads are in flight together: a row of one
+// long sequence has a dozen parts, and each would cost an L2 round trip.
 __global__ void __launch_bounds__(kMergeThreads) attn_merge_kernel(KvCache c, Pass own, Rows ro, Pass pre, Rows rp,
                                                                    float* __restrict__ out) {
+  constexpr int kAhead = 8;
   __shared__ int s_b;
   const int token = blockIdx.x, h = blockIdx.y, group = own.n_heads / c.n_kv_heads, hd = c.head_dim;
-  if (threadIdx.x == 0) {
-    int b = token < own.n_seqs ? token : -1;
-    if (own.q_start) {  // the last sequence that starts at or before the token and has it
-      int lo = 0, hi = own.n_seqs;
+  griddep_wait();
+  griddep_launch_dependents();
+  int b = token < own.n_seqs ? token : -1;
+  if (own.q_start) {  // the last sequence that starts at or before the token and has it
+    if (threadIdx.x < 32) {
+      int lo = 0, hi = own.n_seqs;  // the answer is in [lo, hi): 32 probes a step
       while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (own.q_start[mid] <= token) lo = mid;
-        else hi = mid;
+        const int step = (hi - lo + 31) / 32, at = lo + (int)threadIdx.x * step;
+        const unsigned below = __ballot_sync(0xffffffffu, at < hi && own.q_start[at] <= token);
+        const int last = 31 - __clz((int)below);
+        if (last < 0) break;  // before the first sequence
+        hi = min(hi, lo + (last + 1) * step);
+        lo += last * step;
       }
-      b = own.q_start[lo] <= token && token < own.q_start[lo + 1] ? lo : -1;
+      if (threadIdx.x == 0) s_b = own.q_start[lo] <= token && token < own.q_start[lo + 1] ? lo : -1;
     }
-    s_b = b;
+    __syncthreads();
+    b = s_b;
   }
-  __syncthreads();
-  const int b = s_b;
   if (b < 0) return;
+  struct Source {
+    Seq s;
+    Span n;
+    long long chunk, line;
+  } src[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    if (k == 0 && !pre.prefix) continue;
+    const Pass& p = k ? own : pre;
+    const Rows& w = k ? ro : rp;
+    src[k].s = seq_of(p, k ? b : 0, c.page_shift);
+    src[k].n = span_of(src[k].s, group, c.n_kv_heads, w.rows, w.tt);
+    src[k].chunk = p.line[0];
+    src[k].line = p.line[1 + (k ? b : 0)];
+  }
   for (int i = threadIdx.x; i < group * (hd / 4); i += kMergeThreads) {
     const int hg = i / (hd / 4), d = (i - hg * (hd / 4)) * 4;
     const size_t at = (size_t)token * own.n_heads + (size_t)h * group + hg;
     float top = -INFINITY, sum = 0.f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     bool done = false;
-    for (int k = pre.prefix ? 0 : 1; k < 2; ++k) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (k == 0 && !pre.prefix) continue;
       const Pass& p = k ? own : pre;
       const Rows& w = k ? ro : rp;
-      const int sb = k ? b : 0;
-      const Seq s = seq_of(p, sb, c.page_shift);
-      const Span n = span_of(s, group, c.n_kv_heads, w.rows, w.tt);
-      const int row = (token - s.start) * group + hg;
-      const long long chunk = p.line[0];
-      const long long u0 = p.line[1 + sb] + ((long long)h * n.rt + row / w.rows) * n.tl, u1 = u0 + n.tl;
-      const long long i0 = u0 / chunk, i1 = (u1 - 1) / chunk;
-      if (i0 == i1) {
-        if (!p.ml) {  // finished by its CTA
-          done = true;
-          break;
-        }
-        const float2 e = p.ml[at];
-        join(top, sum, x, e.x, e.y, *reinterpret_cast<const float4*>(p.out + at * hd + d));
-        continue;
+      const Source& q = src[k];
+      const int row = (token - q.s.start) * group + hg, r = row % w.rows;
+      const long long u0 = q.line + ((long long)h * q.n.rt + row / w.rows) * q.n.tl, u1 = u0 + q.n.tl;
+      const int i0 = quotient(u0, (int)q.chunk), i1 = quotient(u1 - 1, (int)q.chunk);
+      if (i0 == i1 && !p.ml) {  // finished by its CTA
+        done = true;
+        break;
       }
-      for (long long ci = i0; ci <= i1; ++ci) {
-        const float* part = p.parts + (size_t)(2 * ci + (ci * chunk > u0 ? 0 : 1)) * w.part;
-        const int r = row % w.rows;
-        const float2 e = *reinterpret_cast<const float2*>(part + w.rows * hd + 2 * r);
-        join(top, sum, x, e.x, e.y, *reinterpret_cast<const float4*>(part + r * hd + d));
+      for (int c0 = i0; c0 <= i1; c0 += kAhead) {
+        float2 e[kAhead];
+        float4 y[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          const int ci = c0 + a;
+          e[a] = make_float2(-INFINITY, 0.f);
+          y[a] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (ci > i1) continue;
+          if (i0 == i1) {  // a whole unit's sums
+            e[a] = p.ml[at];
+            y[a] = *reinterpret_cast<const float4*>(p.out + at * hd + d);
+          } else {
+            const float* part = p.parts + (size_t)(2 * ci + (ci * q.chunk > u0 ? 0 : 1)) * w.part;
+            e[a] = *reinterpret_cast<const float2*>(part + w.rows * hd + 2 * r);
+            y[a] = *reinterpret_cast<const float4*>(part + r * hd + d);
+          }
+        }
+        float mn = top;
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) mn = fmaxf(mn, e[a].x);
+        if (mn == -INFINITY) continue;
+        const float f0 = exp2_approx(top - mn);
+        x.x *= f0, x.y *= f0, x.z *= f0, x.w *= f0;
+        sum *= f0;
+        top = mn;
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          const float f = exp2_approx(e[a].x - mn);
+          x.x = fmaf(y[a].x, f, x.x), x.y = fmaf(y[a].y, f, x.y);
+          x.z = fmaf(y[a].z, f, x.z), x.w = fmaf(y[a].w, f, x.w);
+          sum = fmaf(e[a].y, f, sum);
+        }
       }
     }
     if (done) continue;
@@ -602,10 +686,10 @@ struct Choice {
   Rows rows;
 };
 
-template <int HD, int TYPE, int MT, int TT, int MINB>
+template <int HD, int TYPE, int MT, int TT, int NS, int MINB>
 Choice choice() {
-  using T = Tile<HD, TYPE, MT, TT>;
-  return {attn_tiles_kernel<HD, TYPE, MT, TT, MINB>, T::kSmem, MINB, {T::kRows, TT, T::kPart}};
+  using T = Tile<HD, TYPE, MT, TT, NS>;
+  return {attn_tiles_kernel<HD, TYPE, MT, TT, NS, MINB>, T::kSmem, MINB, {T::kRows, TT, T::kPart}};
 }
 
 // The kernel for units of `rows` query rows.
@@ -613,9 +697,9 @@ template <int HD, int TYPE>
 Choice choose(int rows) {
   constexpr int wide = TYPE == kTypeF16 || HD == 256 ? 16 : 32;
   constexpr int few = HD == 256 ? (TYPE == kTypeF16 ? 1 : 2) : 3;
-  if (rows <= 8) return choice<HD, TYPE, 1, wide, few>();
-  if (rows <= 16 || HD == 256) return choice<HD, TYPE, 2, 16, HD == 256 ? 1 : 3>();
-  return choice<HD, TYPE, HD == 256 ? 2 : 4, 16, HD == 256 ? 1 : 2>();
+  if (rows <= 8) return choice<HD, TYPE, 1, wide, 2, few>();
+  if (rows <= 16 || HD == 256) return choice<HD, TYPE, 2, 16, 2, HD == 256 ? 1 : 3>();
+  return choice<HD, TYPE, HD == 256 ? 2 : 4, 16, 2, HD == 256 ? 1 : 2>();
 }
 
 Choice choose(const KvCache& c, int rows) {
@@ -709,8 +793,18 @@ cudaError_t attn_launch(const KvCache& c, const Attn& a, int sm_count, cudaStrea
     kp.fn<<<kp.per_sm * sm_count, kAttnThreads, kp.smem, s>>>(c, pre);
   }
   ko.fn<<<ko.per_sm * sm_count, kAttnThreads, ko.smem, s>>>(c, own);
-  attn_merge_kernel<<<dim3(a.n_tokens, c.n_kv_heads), kMergeThreads, 0, s>>>(c, own, ko.rows, pre, kp.rows, a.out);
-  return cudaGetLastError();
+  // the merge's CTAs come up while the tiles' drain; they wait for all of it before they read
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.n_tokens, c.n_kv_heads);
+  cfg.blockDim = dim3(kMergeThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaError_t e = cudaGetLastError()) return e;
+  return cudaLaunchKernelEx(&cfg, attn_merge_kernel, c, own, ko.rows, pre, kp.rows, a.out);
 }
 
 }  // namespace gi
