@@ -285,6 +285,30 @@ func (m *Model) Generate(prompt []int32, startPos, n int) ([]uint32, error) {
 	return out, nil
 }
 
+// GenerateSampled is Generate with len(u) tokens picked by temperature, top-k,
+// top-p and min-p (gi_cuda_model_generate_sampled); u holds the picks'
+// uniform numbers in [0, 1).
+func (m *Model) GenerateSampled(prompt []int32, startPos int, u []float32, temperature float32, topK int,
+	topP, minP float32) ([]uint32, error) {
+	out := make([]uint32, len(u))
+	rc := C.gi_cuda_model_generate_sampled(m.h, (*C.int32_t)(&prompt[0]), C.uint32_t(len(prompt)),
+		C.uint32_t(startPos), C.uint32_t(len(u)), C.float(temperature), C.int32_t(topK), C.float(topP),
+		C.float(minP), (*C.float)(&u[0]), (*C.uint32_t)(&out[0]), nil, nil)
+	if rc != 0 {
+		return nil, lastErr("gi_cuda_model_generate_sampled", rc)
+	}
+	return out, nil
+}
+
+// SetKVCache chooses the type of the model's KV cache: GGML type id 0 (F32, the
+// default), 1 (F16) or 8 (Q8_0); empties the cache (gi_cuda_model_set_kv_cache).
+func (m *Model) SetKVCache(quantType int) error {
+	if rc := C.gi_cuda_model_set_kv_cache(m.h, C.int(quantType)); rc != 0 {
+		return lastErr("gi_cuda_model_set_kv_cache", rc)
+	}
+	return nil
+}
+
 // SetPersistent runs every layer of a step in one persistent kernel
 // (gi_cuda_model_set_persistent; Q4_K layers without biases, -2 otherwise).
 func (m *Model) SetPersistent(on bool) error {

@@ -12,6 +12,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <functional>
 #include <mutex>
 #include <string>
 #include <thread>
@@ -377,16 +378,7 @@ void tp_release() {
   g_tp = TpCtx();
 }
 
-struct ModelHandle {
-  gi::DecodeModel m;
-  uint32_t* pinned = nullptr;  // prompt tokens staged for the per-step copies
-  size_t pinned_cap = 0;
-  gi::StepState* pinned_state = nullptr;
-  ~ModelHandle() {
-    if (pinned) cudaFreeHost(pinned);
-    if (pinned_state) cudaFreeHost(pinned_state);
-  }
-};
+using gi::ModelHandle;
 
 const Buffer* as_buffer(gi_cuda_buffer_t b) { return static_cast<const Buffer*>(b); }
 
@@ -455,6 +447,77 @@ int capi_ready(CapiCtx* c) {
 }
 
 int capi_fail(int code, const char* what, cudaError_t e) { return fail(code, what, e); }
+
+int model_generate(ModelHandle* h, const int32_t* tokens, uint32_t n_tokens, uint32_t start_pos, uint32_t n_gen,
+                   const std::function<int(int, cudaStream_t)>& begin, uint32_t* out_tokens, float* out_logits,
+                   float* decode_ms) {
+  gi::DecodeModel& m = h->m;
+  const gi::ModelCfg& c = m.cfg();
+  const uint64_t steps = (uint64_t)n_tokens + n_gen - 1;
+  if ((uint64_t)start_pos + steps > (uint64_t)c.max_pos) return fail(-4, "positions beyond the RoPE table");
+  if (steps > (uint64_t)m.max_out()) return fail(-4, "too many steps for one call");
+  const int64_t full_vocab = (int64_t)c.vocab * c.tp_world;  // the token table is replicated
+  for (uint32_t i = 0; i < n_tokens; ++i)
+    if (tokens[i] < 0 || tokens[i] >= full_vocab) return fail(-4, "token id out of range");
+  if (begin)
+    if (int rc = begin((int)steps, g.stream)) return rc;
+  cudaGraphExec_t& step = m.step_graph();
+  if (!step) {
+    cudaGraph_t graph = nullptr;
+    GI_CUDA_TRY(cudaStreamBeginCapture(g.stream, cudaStreamCaptureModeThreadLocal), "begin capture");
+    const int rc = m.enqueue_step(g.stream, true, true);
+    const cudaError_t ce = cudaStreamEndCapture(g.stream, &graph);
+    if (rc || ce != cudaSuccess) {
+      if (graph) cudaGraphDestroy(graph);
+      return fail(rc ? rc : -5, "capturing the decode step", ce);
+    }
+    const cudaError_t ie = cudaGraphInstantiate(&step, graph, 0);
+    cudaGraphDestroy(graph);
+    if (ie != cudaSuccess) {
+      step = nullptr;
+      return fail(-5, "instantiating the decode step", ie);
+    }
+  }
+  if (h->pinned_cap < n_tokens) {
+    if (h->pinned) cudaFreeHost(h->pinned);
+    h->pinned = nullptr;
+    h->pinned_cap = 0;
+    GI_CUDA_TRY(cudaHostAlloc(reinterpret_cast<void**>(&h->pinned), sizeof(uint32_t) * n_tokens, cudaHostAllocDefault),
+                "pinned prompt");
+    h->pinned_cap = n_tokens;
+  }
+  std::memcpy(h->pinned, tokens, sizeof(uint32_t) * n_tokens);
+  gi::StepState* st = h->pinned_state;
+  *st = gi::StepState();
+  st->token = (uint32_t)tokens[0];
+  st->pos = start_pos;
+  st->slot = start_pos % (uint32_t)c.max_seq;
+  st->active = start_pos + 1 < (uint32_t)c.max_seq ? start_pos + 1 : (uint32_t)c.max_seq;
+  GI_CUDA_TRY(cudaMemcpyAsync(m.state(), st, sizeof *st, cudaMemcpyHostToDevice, g.stream), "copy state");
+  for (uint32_t i = 0; i < n_tokens; ++i) {
+    if (i > 0)  // the argmax just wrote st.token: the prompt overrides it
+      GI_CUDA_TRY(cudaMemcpyAsync(&m.state()->token, h->pinned + i, sizeof(uint32_t), cudaMemcpyHostToDevice,
+                                  g.stream),
+                  "copy prompt token");
+    GI_CUDA_TRY(cudaGraphLaunch(step, g.stream), "decode step");
+  }
+  cudaEvent_t e0 = nullptr, e1 = nullptr;
+  GI_CUDA_TRY(cudaEventCreate(&e0), "event");
+  GI_CUDA_TRY(cudaEventCreate(&e1), "event");
+  cudaEventRecord(e0, g.stream);
+  for (uint32_t i = 1; i < n_gen; ++i) GI_CUDA_TRY(cudaGraphLaunch(step, g.stream), "decode step");
+  cudaEventRecord(e1, g.stream);
+  cudaError_t e = cudaMemcpyAsync(out_tokens, m.tokens_out() + (n_tokens - 1), sizeof(uint32_t) * n_gen,
+                                  cudaMemcpyDeviceToHost, g.stream);
+  if (e == cudaSuccess && out_logits)
+    e = cudaMemcpyAsync(out_logits, m.logits(), sizeof(float) * c.vocab, cudaMemcpyDeviceToHost, g.stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(g.stream);
+  if (e == cudaSuccess && decode_ms) cudaEventElapsedTime(decode_ms, e0, e1);
+  cudaEventDestroy(e0);
+  cudaEventDestroy(e1);
+  if (e != cudaSuccess) return fail(-5, "generate", e);
+  return check_device_error();
+}
 
 }  // namespace gi
 
@@ -933,12 +996,9 @@ int gi_cuda_model_set_persistent(gi_cuda_model_t model, int enable) {
   if (!model) return fail(-4, "null model");
   ModelHandle* h = static_cast<ModelHandle*>(model);
   GI_CUDA_TRY(cudaStreamSynchronize(g.stream), "persistent layers");
-  if (h->m.graph) {  // captured with the other kind of step
-    cudaGraphExecDestroy(h->m.graph);
-    h->m.graph = nullptr;
-  }
+  h->m.drop_graphs();  // captured with the other kind of step
   const int rc = h->m.set_persistent(enable != 0);
-  if (rc == -2) return fail(rc, "persistent layers need Q4_K layer matrices and no biases");
+  if (rc == -2) return fail(rc, "persistent layers need Q4_K layer matrices, no biases and the float32 cache");
   if (rc) return fail(rc, "persistent layer plan", rc == -5 ? cudaGetLastError() : cudaSuccess);
   return 0;
 }
@@ -948,70 +1008,8 @@ int gi_cuda_model_generate(gi_cuda_model_t model, const int32_t* tokens, uint32_
   std::lock_guard<std::mutex> lk(g.mu);
   if (int rc = ensure_ready()) return rc;
   if (!model || !tokens || !out_tokens || n_tokens < 1 || n_gen < 1) return fail(-4, "bad generate arguments");
-  ModelHandle* h = static_cast<ModelHandle*>(model);
-  gi::DecodeModel& m = h->m;
-  const gi::ModelCfg& c = m.cfg();
-  const uint64_t steps = (uint64_t)n_tokens + n_gen - 1;
-  if ((uint64_t)start_pos + steps > (uint64_t)c.max_pos) return fail(-4, "positions beyond the RoPE table");
-  if (steps > (uint64_t)m.max_out()) return fail(-4, "too many steps for one call");
-  const int64_t full_vocab = (int64_t)c.vocab * c.tp_world;  // the token table is replicated
-  for (uint32_t i = 0; i < n_tokens; ++i)
-    if (tokens[i] < 0 || tokens[i] >= full_vocab) return fail(-4, "token id out of range");
-  if (!m.graph) {
-    cudaGraph_t graph = nullptr;
-    GI_CUDA_TRY(cudaStreamBeginCapture(g.stream, cudaStreamCaptureModeThreadLocal), "begin capture");
-    const int rc = m.enqueue_step(g.stream, true, true);
-    const cudaError_t ce = cudaStreamEndCapture(g.stream, &graph);
-    if (rc || ce != cudaSuccess) {
-      if (graph) cudaGraphDestroy(graph);
-      return fail(rc ? rc : -5, "capturing the decode step", ce);
-    }
-    const cudaError_t ie = cudaGraphInstantiate(&m.graph, graph, 0);
-    cudaGraphDestroy(graph);
-    if (ie != cudaSuccess) {
-      m.graph = nullptr;
-      return fail(-5, "instantiating the decode step", ie);
-    }
-  }
-  if (h->pinned_cap < n_tokens) {
-    if (h->pinned) cudaFreeHost(h->pinned);
-    h->pinned = nullptr;
-    h->pinned_cap = 0;
-    GI_CUDA_TRY(cudaHostAlloc(reinterpret_cast<void**>(&h->pinned), sizeof(uint32_t) * n_tokens, cudaHostAllocDefault),
-                "pinned prompt");
-    h->pinned_cap = n_tokens;
-  }
-  std::memcpy(h->pinned, tokens, sizeof(uint32_t) * n_tokens);
-  gi::StepState* st = h->pinned_state;
-  *st = gi::StepState();
-  st->token = (uint32_t)tokens[0];
-  st->pos = start_pos;
-  st->slot = start_pos % (uint32_t)c.max_seq;
-  st->active = start_pos + 1 < (uint32_t)c.max_seq ? start_pos + 1 : (uint32_t)c.max_seq;
-  GI_CUDA_TRY(cudaMemcpyAsync(m.state(), st, sizeof *st, cudaMemcpyHostToDevice, g.stream), "copy state");
-  for (uint32_t i = 0; i < n_tokens; ++i) {
-    if (i > 0)  // the argmax just wrote st.token: the prompt overrides it
-      GI_CUDA_TRY(cudaMemcpyAsync(&m.state()->token, h->pinned + i, sizeof(uint32_t), cudaMemcpyHostToDevice,
-                                  g.stream),
-                  "copy prompt token");
-    GI_CUDA_TRY(cudaGraphLaunch(m.graph, g.stream), "decode step");
-  }
-  cudaEvent_t e0 = nullptr, e1 = nullptr;
-  GI_CUDA_TRY(cudaEventCreate(&e0), "event");
-  GI_CUDA_TRY(cudaEventCreate(&e1), "event");
-  cudaEventRecord(e0, g.stream);
-  for (uint32_t i = 1; i < n_gen; ++i) GI_CUDA_TRY(cudaGraphLaunch(m.graph, g.stream), "decode step");
-  cudaEventRecord(e1, g.stream);
-  cudaError_t e = cudaMemcpyAsync(out_tokens, m.tokens_out() + (n_tokens - 1), sizeof(uint32_t) * n_gen,
-                                  cudaMemcpyDeviceToHost, g.stream);
-  if (e == cudaSuccess && out_logits)
-    e = cudaMemcpyAsync(out_logits, m.logits(), sizeof(float) * c.vocab, cudaMemcpyDeviceToHost, g.stream);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(g.stream);
-  if (e == cudaSuccess && decode_ms) cudaEventElapsedTime(decode_ms, e0, e1);
-  cudaEventDestroy(e0);
-  cudaEventDestroy(e1);
-  if (e != cudaSuccess) return fail(-5, "generate", e);
-  return check_device_error();
+  return gi::model_generate(static_cast<ModelHandle*>(model), tokens, n_tokens, start_pos, n_gen, nullptr,
+                            out_tokens, out_logits, decode_ms);
 }
 
 int gi_cuda_tp_prepare(int world, uint32_t max_dim, void* handle_out) {

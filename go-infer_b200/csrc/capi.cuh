@@ -4,7 +4,10 @@
 
 #include <cuda_runtime.h>
 
+#include <functional>
 #include <mutex>
+
+#include "model.cuh"
 
 namespace gi {
 
@@ -18,6 +21,23 @@ std::mutex& capi_mutex();
 // Binds the calling thread to the library's device (mutex held); a status
 // code, with its text set, when gi_cuda_init has not succeeded.
 int capi_ready(CapiCtx* c);
+// A gi_cuda_model_t.
+struct ModelHandle {
+  DecodeModel m;
+  uint32_t* pinned = nullptr;  // prompt tokens staged for the per-step copies
+  size_t pinned_cap = 0;
+  StepState* pinned_state = nullptr;
+  ~ModelHandle() {
+    if (pinned) cudaFreeHost(pinned);
+    if (pinned_state) cudaFreeHost(pinned_state);
+  }
+};
+
+// gi_cuda_model_generate (mutex held, checked pointers).  begin(steps, stream),
+// if given, sets the steps up after the checks; its status code ends the call.
+int model_generate(ModelHandle* h, const int32_t* tokens, uint32_t n_tokens, uint32_t start_pos, uint32_t n_gen,
+                   const std::function<int(int, cudaStream_t)>& begin, uint32_t* out_tokens, float* out_logits,
+                   float* decode_ms);
 // Sets gi_cuda_last_error's text and returns `code`.
 int capi_fail(int code, const char* what, cudaError_t e = cudaSuccess);
 

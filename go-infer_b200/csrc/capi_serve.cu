@@ -2,7 +2,9 @@
 // batch from a paged KV cache: argument checks and launches.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <mutex>
+#include <vector>
 
 #include "../../include/goinfer_cuda.h"
 #include "capi.cuh"
@@ -222,6 +224,51 @@ int gi_cuda_sample_dev(int32_t* ids, float* prob, const float* logits, size_t lo
   if (!rows) return 0;
   GI_CUDA_TRY(gi::sample_launch(p, ctx.sm_count, stream_of(ctx, stream)), "sampling");
   return 0;
+}
+
+int gi_cuda_model_set_kv_cache(gi_cuda_model_t model, int type) {
+  if (type != GI_TYPE_F32 && type != GI_TYPE_F16 && type != GI_TYPE_Q8_0) return fail(-2, "unsupported cache type");
+  if (!model) return fail(-4, "null model");
+  std::lock_guard<std::mutex> lk(gi::capi_mutex());
+  gi::CapiCtx ctx;
+  if (int rc = serve_ready(&ctx)) return rc;
+  gi::ModelHandle* h = static_cast<gi::ModelHandle*>(model);
+  GI_CUDA_TRY(cudaStreamSynchronize(ctx.stream), "cache type");
+  h->m.drop_graphs();  // captured with the other cache
+  const int rc = h->m.set_kv_cache(type);
+  if (rc == -2) return fail(rc, "the persistent layers need the float32 cache");
+  if (rc == -4) return fail(rc, "F16 and Q8_0 caches take head dims 64, 96, 128 and 256");
+  if (rc) return fail(rc, "cache buffers", cudaGetLastError());
+  h->m.reset_cache(ctx.stream);
+  GI_CUDA_TRY(cudaStreamSynchronize(ctx.stream), "empty cache");
+  return 0;
+}
+
+int gi_cuda_model_generate_sampled(gi_cuda_model_t model, const int32_t* tokens, uint32_t n_tokens,
+                                   uint32_t start_pos, uint32_t n_gen, float temperature, int32_t top_k, float top_p,
+                                   float min_p, const float* u, uint32_t* out_tokens, float* out_logits,
+                                   float* decode_ms) {
+  if (!model || !tokens || !out_tokens || !u || n_tokens < 1 || n_gen < 1) return fail(-4, "bad generate arguments");
+  std::lock_guard<std::mutex> lk(gi::capi_mutex());
+  gi::CapiCtx ctx;
+  if (int rc = serve_ready(&ctx)) return rc;
+  gi::ModelHandle* h = static_cast<gi::ModelHandle*>(model);
+  if (h->m.cfg().vocab > (1 << 20)) return fail(-4, "vocab out of range");
+  gi::StepSampling p;
+  p.temperature = temperature;
+  p.top_k = top_k;
+  p.top_p = top_p;
+  p.min_p = min_p;
+  auto begin = [&](int steps, cudaStream_t s) {
+    std::vector<float> all((size_t)steps, 0.f);  // the prompt's steps pick nothing that is used
+    std::copy(u, u + n_gen, all.begin() + (n_tokens - 1));
+    const int rc = h->m.start_sampling(p, all.data(), steps, s);
+    if (rc == -2) return fail(rc, "sampling under tensor parallelism");
+    return rc ? fail(rc, "sampling buffers", cudaGetLastError()) : 0;
+  };
+  const int rc = gi::model_generate(h, tokens, n_tokens, start_pos, n_gen, begin, out_tokens, out_logits, decode_ms);
+  h->m.stop_sampling();
+  return rc;
 }
 
 }  // extern "C"

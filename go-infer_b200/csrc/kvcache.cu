@@ -204,7 +204,7 @@ void rope_freqs(int scaling, int dim, double theta, double factor, double low, d
   const double first = scaling == GI_ROPE_YARN ? std::fmax(std::floor(pair_of(high)), 0.0) : 0.0;
   const double last = scaling == GI_ROPE_YARN ? std::fmin(std::ceil(pair_of(low)), dim - 1.0) : 0.0;
   for (int i = 0; i < dim / 2; ++i) {
-    const double f = std::pow(theta, -2.0 * i / dim);
+    const double f = 1.0 / std::pow(theta, 2.0 * i / dim);  // as the decode step's table (kernels.go:25-29)
     double r = f;
     if (scaling == GI_ROPE_LINEAR) {
       r = f / factor;

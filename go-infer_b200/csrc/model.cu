@@ -350,6 +350,21 @@ __global__ void __launch_bounds__(1024) argmax_kernel(const float* __restrict__ 
   }
 }
 
+// The sampled pick takes the argmax kernel's place: store it, advance the
+// position, bring up the next step's uniform.
+__global__ void take_pick_kernel(const int32_t* __restrict__ id, StepState* st, uint32_t* __restrict__ out, int max_out,
+                                 int max_seq, const float* __restrict__ u, float* __restrict__ now) {
+  const uint32_t token = (uint32_t)max(*id, 0), n = st->n_out + 1;  // -1: a row without candidates
+  if ((int)st->n_out < max_out) out[st->n_out] = token;
+  st->n_out = n;
+  st->token = token;
+  const uint32_t pos = st->pos + 1;
+  st->pos = pos;
+  st->slot = pos % (uint32_t)max_seq;
+  st->active = pos + 1 < (uint32_t)max_seq ? pos + 1 : (uint32_t)max_seq;
+  if ((int)n < max_out) *now = u[n];
+}
+
 template <typename T>
 int dev_alloc(T** p, size_t n, size_t* total) {
   if (cudaMalloc(reinterpret_cast<void**>(p), sizeof(T) * (n ? n : 1)) != cudaSuccess) return -5;
@@ -370,11 +385,12 @@ float attn_scale_for(int head_dim) {
 }
 
 DecodeModel::~DecodeModel() {
-  if (graph) cudaGraphExecDestroy(graph);
+  drop_graphs();
   layers_plan_free(plan_);
   for (void* p : {(void*)x_, (void*)xb_, (void*)q_, (void*)k_, (void*)v_, (void*)att_, (void*)proj_, (void*)gate_,
                   (void*)up_, (void*)logits_, (void*)kcache_, (void*)vcache_, (void*)part_, (void*)rope_, (void*)st_,
-                  (void*)tokens_out_})
+                  (void*)tokens_out_, (void*)kv_data_, (void*)kv_pages_, (void*)kv_freqs_, (void*)kv_q_, (void*)kv_ws_,
+                  (void*)sample_p_, (void*)sample_u_, (void*)sample_now_, (void*)sample_id_})
     if (p) cudaFree(p);
   delete[] layers_;
 }
@@ -462,12 +478,116 @@ int DecodeModel::set_persistent(bool on) {
   layers_plan_free(plan_);
   plan_ = nullptr;
   if (!on) return 0;
+  if (kv_type_ != kTypeF32) return -2;
   if (int rc = layers_prepare_device()) return rc;
   return layers_plan_build(layers_, n_layers_, cfg_, x_, q_, k_, v_, att_, gate_, up_,
                            cfg_.tp_world > 1 ? &tp_ : nullptr, sm_count_, &plan_);
 }
 
+int DecodeModel::set_kv_cache(int type) {
+  if (type == kv_type_) return 0;
+  if ((type != kTypeF32 && type != kTypeF16 && type != kTypeQ8_0) || plan_) return -2;
+  const ModelCfg& c = cfg_;
+  if (type != kTypeF32 && !attn_head_dim_ok(c.head_dim)) return -4;
+  size_t t = 0;
+  if (type == kTypeF32) {
+    const size_t n = (size_t)c.n_layers * c.max_seq * c.n_kv_heads * c.head_dim;
+    float *k = nullptr, *v = nullptr;
+    if (dev_alloc(&k, n, &t) || dev_alloc(&v, n, &t)) {
+      if (k) cudaFree(k);
+      return -5;
+    }
+    kcache_ = k;
+    vcache_ = v;
+    cudaFree(kv_data_);
+    kv_data_ = nullptr;
+    kv_type_ = type;
+    return 0;
+  }
+  KvCache kv;
+  kv.type = type;
+  kv.n_kv_heads = c.n_kv_heads;
+  kv.head_dim = c.head_dim;
+  kv.page_size = 64;
+  kv.page_shift = 6;
+  kv.n_pages = (c.max_seq + kv.page_size - 1) / kv.page_size;
+  int64_t at[4];
+  const size_t layer = (size_t)kv_cache_layout(type, kv.n_pages, kv.page_size, kv.n_kv_heads, kv.head_dim, at);
+  Attn a;
+  a.n_heads = c.n_heads;
+  a.max_tokens = a.max_q_len = 1;
+  a.scale = c.attn_scale;
+  uint8_t* data = nullptr;
+  if (dev_alloc(&data, layer * c.n_layers, &t)) return -5;
+  if (!kv_pages_) {  // the first time: what does not depend on the type
+    std::vector<int32_t> pages(kv.n_pages);
+    for (int i = 0; i < kv.n_pages; ++i) pages[i] = i;
+    std::vector<double> freqs(c.head_dim / 2);
+    double mscale = 1.0;
+    rope_freqs(0, c.head_dim, (double)c.rope_theta, 1.0, 1.0, 4.0, 1.0, freqs.data(), &mscale);
+    KvCache any = kv;
+    const size_t ws16 = (any.type = kTypeF16, attn_workspace(any, a, sm_count_));
+    const size_t ws8 = (any.type = kTypeQ8_0, attn_workspace(any, a, sm_count_));
+    int32_t* p = nullptr;
+    int rc = dev_alloc(&p, kv.n_pages, &t);
+    if (!rc && !kv_freqs_) rc = dev_alloc(&kv_freqs_, freqs.size(), &t);
+    if (!rc && !kv_q_) rc = dev_alloc(&kv_q_, (size_t)c.n_heads * c.head_dim, &t);
+    if (!rc && !kv_ws_) rc = dev_alloc(&kv_ws_, ws16 > ws8 ? ws16 : ws8, &t);
+    if (!rc && (cudaMemcpy(p, pages.data(), sizeof(int32_t) * pages.size(), cudaMemcpyHostToDevice) != cudaSuccess ||
+                cudaMemcpy(kv_freqs_, freqs.data(), sizeof(double) * freqs.size(), cudaMemcpyHostToDevice) !=
+                    cudaSuccess))
+      rc = -5;
+    if (rc) {
+      if (p) cudaFree(p);
+      cudaFree(data);
+      return -5;
+    }
+    kv_pages_ = p;
+  }
+  kv.k = data + at[0];
+  kv.v = data + at[1];
+  kv.ks = reinterpret_cast<__half*>(data + at[2]);
+  kv.vs = reinterpret_cast<__half*>(data + at[3]);
+  for (void* old : {(void*)kcache_, (void*)vcache_, (void*)kv_data_})
+    if (old) cudaFree(old);
+  kcache_ = vcache_ = nullptr;
+  kv_ = kv;
+  kv_data_ = data;
+  kv_layer_bytes_ = layer;
+  kv_type_ = type;
+  a.out = att_;
+  a.q = kv_q_;
+  a.n_seqs = a.n_tokens = 1;
+  a.kv_len = reinterpret_cast<const int32_t*>(&st_->active);
+  a.pages = kv_pages_;
+  a.pages_stride = kv.n_pages;
+  a.ws = kv_ws_;
+  kv_attn_ = a;
+  return 0;
+}
+
+int DecodeModel::start_sampling(const StepSampling& p, const float* u, int n, cudaStream_t s) {
+  if (cfg_.tp_world > 1) return -2;
+  if (!sample_id_) {
+    size_t t = 0;
+    if ((!sample_p_ && dev_alloc(&sample_p_, 1, &t)) || (!sample_u_ && dev_alloc(&sample_u_, max_out_, &t)) ||
+        (!sample_now_ && dev_alloc(&sample_now_, 1, &t)) || dev_alloc(&sample_id_, 1, &t))
+      return -5;
+  }
+  // pageable sources: the copies have read them when they return
+  if (cudaMemcpyAsync(sample_p_, &p, sizeof p, cudaMemcpyHostToDevice, s) != cudaSuccess ||
+      cudaMemcpyAsync(sample_u_, u, sizeof(float) * n, cudaMemcpyHostToDevice, s) != cudaSuccess ||
+      cudaMemcpyAsync(sample_now_, u, sizeof(float), cudaMemcpyHostToDevice, s) != cudaSuccess)
+    return -5;
+  sampling_ = true;
+  return 0;
+}
+
 void DecodeModel::reset_cache(cudaStream_t s) {
+  if (kv_type_ != kTypeF32) {
+    cudaMemsetAsync(kv_data_, 0, kv_layer_bytes_ * cfg_.n_layers, s);
+    return;
+  }
   const size_t kv = (size_t)cfg_.n_layers * cfg_.max_seq * cfg_.n_kv_heads * cfg_.head_dim;
   cudaMemsetAsync(kcache_, 0, sizeof(float) * kv, s);
   cudaMemsetAsync(vcache_, 0, sizeof(float) * kv, s);
@@ -567,16 +687,30 @@ int DecodeModel::enqueue_step(cudaStream_t s, bool embed, bool pdl) {
     if (Ly.bk && e == cudaSuccess) e = launch(pdl, blocks(kv_dim, 256), dim3(256), 0, s, add_kernel, k_, Ly.bk, kv_dim);
     if (Ly.bv && e == cudaSuccess) e = launch(pdl, blocks(kv_dim, 256), dim3(256), 0, s, add_kernel, v_, Ly.bv, kv_dim);
     if (e != cudaSuccess) return -5;
-    // at least two items per SM: under tensor parallelism a rank's few kv
-    // heads are split by query-head groups
-    const int hq = attn_heads_per_item(kv_mul, c.n_kv_heads, att_splits_, 2 * sm_count_);
-    e = launch(pdl, dim3(c.n_kv_heads * (kv_mul / hq), att_splits_), dim3(256), attn_smem_bytes(hq, hd), s,
-               attn_partial_kernel,
-               (const StepState*)st_, (const float*)q_, (const float*)k_, (const float*)v_, (const float2*)rope_, kc,
-               vc, part_, kv_mul, hd, kv_dim, att_splits_, c.attn_scale, (uint32_t)c.max_pos, scratch_.error, hq);
-    if (e != cudaSuccess) return -5;
-    e = launch(pdl, dim3(c.n_heads), dim3(hd), 0, s, attn_combine_kernel, (const float*)part_, att_, hd, att_splits_);
-    if (e != cudaSuccess) return -5;
+    if (kv_type_ != kTypeF32) {  // rotate, write and read the F16 / Q8_0 cache
+      KvCache lc = kv_;
+      const size_t off = (size_t)l * kv_layer_bytes_;
+      lc.k += off, lc.v += off;
+      lc.ks += off / sizeof(__half), lc.vs += off / sizeof(__half);
+      Rope rope;
+      rope.dim = hd;
+      rope.freqs = kv_freqs_;
+      e = kv_write_launch(lc, k_, kv_dim, v_, kv_dim, reinterpret_cast<const int32_t*>(&st_->slot), 1, q_, q_dim,
+                          kv_q_, c.n_heads, reinterpret_cast<const int32_t*>(&st_->pos), rope, sm_count_, s);
+      if (e == cudaSuccess) e = attn_launch(lc, kv_attn_, sm_count_, s);
+      if (e != cudaSuccess) return -5;
+    } else {
+      // at least two items per SM: under tensor parallelism a rank's few kv
+      // heads are split by query-head groups
+      const int hq = attn_heads_per_item(kv_mul, c.n_kv_heads, att_splits_, 2 * sm_count_);
+      e = launch(pdl, dim3(c.n_kv_heads * (kv_mul / hq), att_splits_), dim3(256), attn_smem_bytes(hq, hd), s,
+                 attn_partial_kernel,
+                 (const StepState*)st_, (const float*)q_, (const float*)k_, (const float*)v_, (const float2*)rope_, kc,
+                 vc, part_, kv_mul, hd, kv_dim, att_splits_, c.attn_scale, (uint32_t)c.max_pos, scratch_.error, hq);
+      if (e != cudaSuccess) return -5;
+      e = launch(pdl, dim3(c.n_heads), dim3(hd), 0, s, attn_combine_kernel, (const float*)part_, att_, hd, att_splits_);
+      if (e != cudaSuccess) return -5;
+    }
     // Output projection + residual (x += Wo att); across ranks the partial
     // products are summed first.
     if (c.tp_world > 1) {
@@ -645,6 +779,23 @@ int DecodeModel::enqueue_step(cudaStream_t s, bool embed, bool pdl) {
   if (e != cudaSuccess) return -5;
   rc = gemv_launch(out_.qtype, logits_, xb_, out_.w, out_.bytes, c.vocab, c.dim, scratch_, L, s);
   if (rc) return rc;
+  if (sampling_) {
+    Sample p;
+    p.ids = sample_id_;
+    p.logits = logits_;
+    p.stride = (size_t)c.vocab;
+    p.rows = 1;
+    p.vocab = c.vocab;
+    p.u = sample_now_;
+    p.temperature = &sample_p_->temperature;
+    p.top_k = &sample_p_->top_k;
+    p.top_p = &sample_p_->top_p;
+    p.min_p = &sample_p_->min_p;
+    e = sample_launch(p, sm_count_, s);
+    if (e != cudaSuccess) return -5;
+    take_pick_kernel<<<1, 1, 0, s>>>(sample_id_, st_, tokens_out_, max_out_, c.max_seq, sample_u_, sample_now_);
+    return cudaGetLastError() == cudaSuccess ? 0 : -5;
+  }
   e = launch(pdl, dim3(1), dim3(1024), 0, s, argmax_kernel, (const float*)logits_, c.vocab, st_, tokens_out_,
              max_out_, c.max_seq, c.vocab_offset, tp_, scratch_.error);
   return e == cudaSuccess ? 0 : -5;

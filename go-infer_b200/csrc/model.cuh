@@ -8,6 +8,7 @@
 #include <stdint.h>
 
 #include "gemv.cuh"
+#include "serve.cuh"
 #include "tp.cuh"
 
 namespace gi {
@@ -43,6 +44,13 @@ struct ModelCfg {
   int tp_world = 1, tp_rank = 0, vocab_offset = 0;
 };
 
+// How the next token is picked: device scalars, one row.
+struct StepSampling {
+  float temperature = 1.f;
+  int32_t top_k = 0;
+  float top_p = 1.f, min_p = 0.f;
+};
+
 // Position state the captured step reads and advances on the device.
 struct StepState {
   uint32_t token;   // input token of the next step
@@ -73,6 +81,18 @@ class DecodeModel {
   // layout does not fit, -5 on a CUDA error.  Off by default.
   int set_persistent(bool on);
   bool persistent() const { return plan_ != nullptr; }
+  // Cache type of each layer's K and V: kTypeF32 (the rolling float32 cache
+  // of attn.cuh, the default), kTypeF16 or kTypeQ8_0 (kvcache.cu, with
+  // paged_attn.cu reading it).  Empties the cache.  -2 for another type or
+  // while the persistent kernel is on, -4 for a head dim that paged_attn.cu
+  // does not have, -5 on a CUDA error (the old cache then stays).
+  int set_kv_cache(int type);
+  int kv_type() const { return kv_type_; }
+  // Steps enqueued from now on pick the token by `p` and the uniforms u[0 ..
+  // n) of the call's steps, or (off) the first maximum.  0, -2 under tensor
+  // parallelism, -5 on a CUDA error.
+  int start_sampling(const StepSampling& p, const float* u, int n, cudaStream_t s);
+  void stop_sampling() { sampling_ = false; }
 
   const ModelCfg& cfg() const { return cfg_; }
   float* x() const { return x_; }
@@ -83,8 +103,14 @@ class DecodeModel {
   size_t device_bytes() const { return dev_bytes_; }
 
   // The captured step (built on first use, replayed per token).
-  cudaGraphExec_t graph = nullptr;
+  cudaGraphExec_t graph = nullptr, graph_sampled = nullptr;
   bool graph_pdl = false;
+  cudaGraphExec_t& step_graph() { return sampling_ ? graph_sampled : graph; }
+  void drop_graphs() {
+    if (graph) cudaGraphExecDestroy(graph);
+    if (graph_sampled) cudaGraphExecDestroy(graph_sampled);
+    graph = graph_sampled = nullptr;
+  }
 
  private:
   ModelCfg cfg_;
@@ -106,6 +132,22 @@ class DecodeModel {
   int att_splits_ = 1;
   size_t dev_bytes_ = 0;
   LayersPlan* plan_ = nullptr;
+  // F16 / Q8_0 cache: every layer's pages in one block, the page table (page i
+  // is i), rotary frequencies, rotated queries, the attention's workspace
+  int kv_type_ = kTypeF32;
+  KvCache kv_;  // layer 0's
+  size_t kv_layer_bytes_ = 0;
+  uint8_t* kv_data_ = nullptr;
+  int32_t* kv_pages_ = nullptr;
+  double* kv_freqs_ = nullptr;
+  float* kv_q_ = nullptr;
+  uint8_t* kv_ws_ = nullptr;
+  Attn kv_attn_;
+  // sampling: the parameters, the uniforms of a call's steps and the present one, the pick
+  bool sampling_ = false;
+  StepSampling* sample_p_ = nullptr;
+  float *sample_u_ = nullptr, *sample_now_ = nullptr;
+  int32_t* sample_id_ = nullptr;
 };
 
 // attn_scale of forward.go:33: float32(1 / math_sqrt(headDim)) with the

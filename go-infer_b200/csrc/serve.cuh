@@ -5,10 +5,11 @@
 // cudaError_t of the launch.
 #pragma once
 
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
+
+struct __half;  // cuda_fp16.h
 
 namespace gi {
 

@@ -55,7 +55,7 @@ EXPORTS = (
     "gi_cuda_model_reset", "gi_cuda_model_set_persistent", "gi_cuda_model_generate", "gi_cuda_tp_prepare", "gi_cuda_tp_connect", "gi_cuda_tp_close",
     "gi_cuda_alloc_buffer", "gi_synth_weights", "gi_cuda_buffer_read",
     "gi_kv_cache_bytes", "gi_rope_freqs", "gi_cuda_kv_write_dev", "gi_cuda_kv_read_dev", "gi_cuda_attn_workspace",
-    "gi_cuda_attn_dev", "gi_cuda_sample_dev",
+    "gi_cuda_attn_dev", "gi_cuda_sample_dev", "gi_cuda_model_set_kv_cache", "gi_cuda_model_generate_sampled",
 )
 
 
@@ -185,6 +185,10 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
         "gi_cuda_kv_read_dev": ([vp, vp, vp, vp, u32, vp], i32),
         "gi_cuda_attn_workspace": ([vp, vp], i64),
         "gi_cuda_attn_dev": ([vp, vp, vp, vp, u32, u32, vp, vp, vp, u32, vp, vp, sz, vp], i32),
+        "gi_cuda_model_set_kv_cache": ([vp, i32], i32),
+        "gi_cuda_model_generate_sampled": ([vp, ctypes.POINTER(ctypes.c_int32), u32, u32, u32, ctypes.c_float,
+                                            ctypes.c_int32, ctypes.c_float, ctypes.c_float, f32p,
+                                            ctypes.POINTER(u32), f32p, f32p], i32),
         "gi_cuda_sample_dev": ([vp, vp, vp, sz, u32, u32, vp, vp, vp, vp, vp, vp], i32),
     }
     for name, (args, res) in sig.items():
@@ -667,6 +671,24 @@ class Model:
             out.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32)), _f32(logits) if logits is not None else None,
             ctypes.byref(ms)))
         return out, logits, ms.value
+
+    def generate_sampled(self, tokens, u, start_pos: int = 0, temperature: float = 1.0, top_k: int = 0,
+                         top_p: float = 1.0, min_p: float = 0.0, want_logits: bool = False):
+        """generate with len(u) tokens picked by sample_dev's rule, u being the picks' uniform numbers."""
+        toks = np.ascontiguousarray(tokens, np.int32)
+        u = np.ascontiguousarray(u, np.float32)
+        out = np.empty(u.size, np.uint32)
+        logits = np.empty(self.vocab, np.float32) if want_logits else None
+        ms = ctypes.c_float(0.0)
+        _err("gi_cuda_model_generate_sampled", load_library().gi_cuda_model_generate_sampled(
+            self.handle, toks.ctypes.data_as(ctypes.POINTER(ctypes.c_int32)), toks.size, start_pos, u.size, temperature,
+            top_k, top_p, min_p, _f32(u), out.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32)),
+            _f32(logits) if logits is not None else None, ctypes.byref(ms)))
+        return out, logits, ms.value
+
+    def set_kv_cache(self, kind: int) -> None:
+        """TYPE_F32 (the default), TYPE_F16 or TYPE_Q8_0; empties the cache."""
+        _err("gi_cuda_model_set_kv_cache", load_library().gi_cuda_model_set_kv_cache(self.handle, kind))
 
     def reset(self) -> None:
         _err("gi_cuda_model_reset", load_library().gi_cuda_model_reset(self.handle))

@@ -1,4 +1,4 @@
-"""Command-line runner: greedy decode of a synthetic Llama-shaped model, or
+"""Command-line runner: greedy or sampled decode of a synthetic Llama-shaped model, or
 one prefill dequant-GEMM, on one GPU.
 
 The counterpart of go-infer's `go-infer run` for this engine's path: it
@@ -9,6 +9,7 @@ generated token.
 
     python go-infer_b200/run.py decode --model llama2-7b --prompt 128 --steps 64
     python go-infer_b200/run.py decode --model llama3-70b --prompt 40 --steps 2
+    python go-infer_b200/run.py decode --model llama2-7b --kv q8_0 --temperature 0.8 --top-k 40 --top-p 0.95
     python go-infer_b200/run.py decode --gguf model.gguf --prompt 16 --steps 32
     python go-infer_b200/run.py export --model llama2-7b --layers 2 --out small.gguf
     python go-infer_b200/run.py prefill --type q4_k --rows 4096 --cols 4096 --batch 512 --reps 3
@@ -29,6 +30,7 @@ import goinfer_cuda as G  # noqa: E402
 import synth  # noqa: E402
 
 MODELS = {"llama2-7b": synth.LLAMA2_7B, "llama3-70b": synth.LLAMA3_70B}
+KV_TYPES = {"f32": G.TYPE_F32, "f16": G.TYPE_F16, "q8_0": G.TYPE_Q8_0}
 TYPES = {"q4_k": G.TYPE_Q4_K, "q6_k": G.TYPE_Q6_K, "q8_0": G.TYPE_Q8_0}
 
 
@@ -49,8 +51,15 @@ def decode(args) -> None:
     try:
         if args.persistent:
             model.set_persistent(True)
+        if args.kv != "f32":
+            model.set_kv_cache(KV_TYPES[args.kv])
         prompt = np.random.default_rng(args.seed * 10).integers(0, cfg.vocab, args.prompt).astype(np.int32)
-        ids, _logits, ms = model.generate(prompt, args.steps)
+        if args.temperature > 0:
+            u = np.random.default_rng(args.seed * 10 + 1).random(args.steps, np.float32)
+            ids, _logits, ms = model.generate_sampled(prompt, u, temperature=args.temperature, top_k=args.top_k,
+                                                      top_p=args.top_p, min_p=args.min_p)
+        else:
+            ids, _logits, ms = model.generate(prompt, args.steps)
         per = ms / max(args.steps - 1, 1)
         print(f"ids {ids.tolist()}")
         print(f"decode {per * 1e3:.1f} us/token ({1e3 / per:.1f} tok/s) over {args.steps - 1} steps")
@@ -148,6 +157,11 @@ def main() -> None:
     d.add_argument("--seed", type=int, default=4)
     d.add_argument("--gguf", default="", help="decode the model of this GGUF file instead")
     d.add_argument("--persistent", action="store_true", help="every layer of a step in one persistent launch")
+    d.add_argument("--kv", choices=sorted(KV_TYPES), default="f32", help="type of the KV cache")
+    d.add_argument("--temperature", type=float, default=0.0, help="sample the tokens (0: greedy)")
+    d.add_argument("--top-k", type=int, default=0)
+    d.add_argument("--top-p", type=float, default=1.0)
+    d.add_argument("--min-p", type=float, default=0.0)
     x = sub.add_parser("export")
     x.add_argument("--model", choices=sorted(MODELS), default="llama2-7b")
     x.add_argument("--layers", type=int, default=0, help="override the layer count")

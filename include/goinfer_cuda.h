@@ -467,6 +467,15 @@ int gi_cuda_attn_dev(const gi_cuda_kv_cache_t* cache, const gi_cuda_attn_t* attn
                      const int32_t* pages, uint32_t pages_stride, const int32_t* prefix_pages, void* workspace,
                      size_t workspace_bytes, void* stream);
 
+/* The cache of a model's decode steps: GI_TYPE_F32 (0, the default: the
+ * rolling float32 cache), GI_TYPE_F16 or GI_TYPE_Q8_0 (half, or a quarter
+ * and a sixteenth, of its size), written and read by the calls above
+ * (kvcache.go's cache types).  Changing the type empties the cache; the step
+ * is captured again at the next generate.  -2 for another type or while the
+ * persistent layers are on, -4 for a head dim that gi_cuda_attn_dev does not
+ * take. */
+int gi_cuda_model_set_kv_cache(gi_cuda_model_t model, int type);
+
 /* The next token of each of `rows` rows of logits (vocab values each,
  * logits_stride floats apart, vocab up to 2^20) by a uniform number u[row] in
  * [0, 1).  Candidates are the logits above -inf (NaN is none).  In the order
@@ -483,6 +492,16 @@ int gi_cuda_attn_dev(const gi_cuda_kv_cache_t* cache, const gi_cuda_attn_t* attn
 int gi_cuda_sample_dev(int32_t* ids, float* prob, const float* logits, size_t logits_stride, uint32_t rows,
                        uint32_t vocab, const float* u, const float* temperature, const int32_t* top_k,
                        const float* top_p, const float* min_p, void* stream);
+
+/* gi_cuda_model_generate with every generated token picked by
+ * gi_cuda_sample_dev's rule from the step's logits: u[0 .. n_gen) (host) are
+ * the uniform numbers of the n_gen picks, out_logits the logits of the last.
+ * One captured graph per step, as the greedy loop.  -2 for a tensor-parallel
+ * model. */
+int gi_cuda_model_generate_sampled(gi_cuda_model_t model, const int32_t* tokens, uint32_t n_tokens,
+                                   uint32_t start_pos, uint32_t n_gen, float temperature, int32_t top_k, float top_p,
+                                   float min_p, const float* u, uint32_t* out_tokens, float* out_logits,
+                                   float* decode_ms);
 
 #ifdef __cplusplus
 }

@@ -152,3 +152,12 @@ def test_plain_sampler_draws_the_shares():
     assert {sample(x, u, 1.0, 0, 0.5, 0.0)[0] for u in grid} == {3}
     assert {sample(x, u, 1.0, 0, 1.0, 0.3)[0] for u in grid} == {1, 3, 4}
     assert sample(x, 0.9, 0.0, 0, 1.0, 0.0) == (3, 1.0) and sample([-math.inf] * 3, 0.5, 1.0, 0, 1.0, 0.0) == (-1, 0.0)
+
+
+def test_model_refusals_without_a_model():
+    lib = G.load_library()
+    assert lib.gi_cuda_model_set_kv_cache(None, G.TYPE_F16) == G.ERR_SHAPE
+    assert lib.gi_cuda_model_set_kv_cache(None, 2) == G.ERR_UNSUPPORTED_TYPE
+    toks, out = (G.ctypes.c_int32 * 1)(1), (G.ctypes.c_uint32 * 1)()
+    u = (G.ctypes.c_float * 1)(0.5)
+    assert lib.gi_cuda_model_generate_sampled(None, toks, 1, 0, 1, 1.0, 0, 1.0, 0.0, u, out, None, None) == G.ERR_SHAPE

@@ -535,3 +535,103 @@ def test_a_batch_is_served_step_by_step(kind):
         for r in range(seqs):
             assert ids[r].item() == sample(x[r], u[r].item(), [0.7, 1.3, 0.0][r] and float(np.float32([0.7, 1.3, 0.0][r])),
                                            0, [0.9, 1.0, 1.0][r], 0.0)[0]
+
+
+# ---- the model's own paths ----------------------------------------------------------------
+
+@pytest.fixture(scope="module")
+def model_host():
+    import synth
+    cfg = synth.LlamaConfig(n_layers=2, dim=512, hidden=1024, n_heads=8, n_kv_heads=2, vocab=1000, max_seq=48)
+    return synth.synth_model(cfg, seed=11)
+
+
+@pytest.fixture()
+def model(model_host):
+    import synth
+    dev = synth.DeviceModel(model_host)
+    m = dev.model()
+    yield m
+    m.close()
+    dev.close()
+
+
+PROMPT = [3, 141, 59, 26, 535]
+
+
+def test_model_samples_from_its_logits(model):
+    """Step by step, each pick follows the rule from the logits the step returns; one call of all steps picks the same."""
+    u = np.random.default_rng(5).random(12, np.float32)
+    kw = dict(temperature=0.9, top_k=50, top_p=0.95, min_p=0.01)
+    ids, _, _ = model.generate_sampled(PROMPT, u, **kw)
+    model.reset()
+    tokens, pos, got = list(PROMPT), 0, []
+    for x in u:
+        one, logits, _ = model.generate_sampled(tokens, [x], start_pos=pos, want_logits=True, **kw)
+        assert one[0] == sample(logits, float(x), float(np.float32(0.9)), 50, 0.95, 0.01)[0]
+        pos += len(tokens)
+        tokens = [int(one[0])]
+        got.append(int(one[0]))
+    assert got == ids.tolist() and len(set(got)) > 3
+
+
+def test_model_sampled_without_choice_is_greedy(model):
+    greedy, logits, _ = model.generate(PROMPT, 20, want_logits=True)
+    for kw in (dict(temperature=0.0), dict(top_k=1), dict(top_p=0.0), dict(min_p=1.0)):
+        model.reset()
+        ids, x, _ = model.generate_sampled(PROMPT, np.full(20, 0.999, np.float32), want_logits=True, **kw)
+        assert np.array_equal(ids, greedy) and np.array_equal(x, logits)
+    model.reset()
+    assert np.array_equal(model.generate(PROMPT, 20)[0], greedy)
+
+
+@pytest.mark.parametrize("kind,tol", [(G.TYPE_F16, 2.0 ** -8), (G.TYPE_Q8_0, 2.0 ** -4)])
+def test_model_with_a_small_cache(model, kind, tol):
+    """Logits of the F16 / Q8_0 cache near the float32 cache's, also past the cache's end (rolling).
+
+    A cached value is off by 2^-11 of itself (F16) or by 1/254 of its block's largest, about 2^-6.5 of a
+    typical value (Q8_0).  Through V that is the attention output's error; through K it moves a score by as
+    much of its size (about 1 here) and so a weight by as much: twice 2^-11, or 2^-6.5 and less after
+    averaging, per layer of 2, of an output that is then added to a residual of its size."""
+    tokens = np.random.default_rng(7).integers(0, 1000, 70)
+    for n in (1, 33, 70):
+        model.set_kv_cache(G.TYPE_F32)
+        _, want, _ = model.generate(tokens[:n], 1, want_logits=True)
+        model.set_kv_cache(kind)
+        first, got, _ = model.generate(tokens[:n], 1, want_logits=True)
+        assert np.sqrt(np.mean((got - want) ** 2)) <= tol * np.sqrt(np.mean(want ** 2))
+        model.reset()
+        again, same, _ = model.generate(tokens[:n], 1, want_logits=True)
+        assert np.array_equal(same, got) and first[0] == again[0] == np.argmax(got)
+
+
+def test_model_cache_refusals(model, model_host):
+    for kind in (2, G.TYPE_Q4_K):
+        with pytest.raises(G.GoInferCudaError) as e:
+            model.set_kv_cache(kind)
+        assert e.value.code == G.ERR_UNSUPPORTED_TYPE
+    model.set_kv_cache(G.TYPE_Q8_0)
+    with pytest.raises(G.GoInferCudaError) as e:
+        model.set_persistent(True)
+    assert e.value.code == G.ERR_UNSUPPORTED_TYPE and "float32 cache" in str(e.value)
+    model.set_kv_cache(G.TYPE_F32)
+    model.set_persistent(True)
+    with pytest.raises(G.GoInferCudaError) as e:
+        model.set_kv_cache(G.TYPE_F16)
+    assert e.value.code == G.ERR_UNSUPPORTED_TYPE
+    greedy, _, _ = model.generate(PROMPT, 5)
+    model.reset()
+    assert np.array_equal(model.generate_sampled(PROMPT, np.zeros(5, np.float32), top_k=1)[0], greedy)
+    model.set_persistent(False)
+    with pytest.raises(G.GoInferCudaError):
+        model.generate_sampled([], [0.5])
+    import synth
+    cfg = synth.LlamaConfig(n_layers=1, dim=256, hidden=512, n_heads=8, n_kv_heads=2, vocab=300, max_seq=16)
+    dev = synth.DeviceModel(synth.synth_model(cfg, seed=3))  # heads of 32
+    m = dev.model()
+    with pytest.raises(G.GoInferCudaError) as e:
+        m.set_kv_cache(G.TYPE_F16)
+    assert e.value.code == G.ERR_SHAPE
+    assert len(m.generate([1, 2], 3)[0]) == 3
+    m.close()
+    dev.close()
