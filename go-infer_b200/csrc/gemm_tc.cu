@@ -59,6 +59,7 @@
 
 #include "common.cuh"
 #include "gemm.cuh"
+#include "tc.cuh"
 
 namespace gi {
 namespace tc {
@@ -68,7 +69,6 @@ constexpr int kTileTok = 128;   // tokens per CTA: MMA N
 constexpr int kTileBytes = 128 * 64 * 2;  // 128 x 64 fp16 operand tile, 128-byte swizzle
 constexpr int kSmallBytes = 128 * 16 * 2;  // 128 x 16 fp16 operand tile, no swizzle
 constexpr int kThreads = 320;
-constexpr uint64_t kWaitNs = 2000000000ull;  // 2 s: far beyond any legitimate wait
 
 // Tensor memory (512 columns x 128 lanes of 32 bits): two D1 accumulator
 // buffers of 128 columns (one per super-block in flight), for Q4_K one D2
@@ -121,201 +121,10 @@ constexpr int smem_bytes() {
   return Cfg<QT>::kStages * stage_bytes<QT, P2>() + 1024 /* alignment */ + 256 /* barriers */;
 }
 
-// ---- tcgen05 / TMA / timer primitives ---------------------------------------
-
-GI_DEVINL uint64_t globaltimer_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-
-// mbarrier test with acquire at cluster scope: for barriers that the other
-// CTA of a pair arrives on.
-GI_DEVINL bool mbar_try_wait_cl(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; "
-      "selp.u32 %0, 1, 0, p; }"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-// Wait for the phase of `parity` on an mbarrier, giving up after kWaitNs
-// (CL: acquire at cluster scope).
-template <bool CL = false>
-GI_DEVINL bool wait_phase(uint32_t bar, uint32_t parity) {
-  auto test = [&]() { return CL ? mbar_try_wait_cl(bar, parity) : mbar_try_wait(bar, parity); };
-  if (test()) return true;
-  const uint64_t t0 = globaltimer_ns();
-  for (;;) {
-    for (int i = 0; i < 32; ++i)
-      if (test()) return true;
-    if (globaltimer_ns() - t0 > kWaitNs) return false;
-  }
-}
-
-// The same for a whole warp: lane 0 polls, every lane gets the outcome, and
-// the warp leaves converged (the tcgen05 .sync.aligned forms require it).
-template <bool CL = false>
-GI_DEVINL bool warp_wait_phase(uint32_t bar, uint32_t parity) {
-  int ok = 0;
-  if ((threadIdx.x & 31) == 0) ok = wait_phase<CL>(bar, parity);
-  return __shfl_sync(0xffffffffu, ok, 0) != 0;
-}
-
-GI_DEVINL void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
-// Contiguous global -> shared bulk copy into this CTA only; completes `bytes`
-// of tx on `bar`.  Both addresses 16-byte aligned, bytes a multiple of 16.
-GI_DEVINL void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-               "l"(src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-
-GI_DEVINL void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-GI_DEVINL void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// D[tmem] (+)= A[smem desc] * B[smem desc]^T, fp16 inputs, fp32 accumulate.
-GI_DEVINL void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{ .reg .pred p; setp.ne.b32 p, %4, 0; "
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// The same with A read from tensor memory (lane m = row m of A, 16-bit
-// column k = element k: two K values per 32-bit column).
-GI_DEVINL void mma_f16_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{ .reg .pred p; setp.ne.b32 p, %4, 0; "
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
-      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// 32 lanes x 32 columns of 32 bits into tensor memory (the warp's lane
-// quarter); completion is awaited with tmem_wait_st.
-GI_DEVINL void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]),
-      "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
-      "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
-GI_DEVINL void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// Arrive once on `bar` when every MMA this thread issued so far has finished.
-GI_DEVINL void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-               : "memory");
-}
-
-// ---- CTA-pair (cta_group::2) forms ------------------------------------------
-// The pair is a cluster of two CTAs; rank 0 issues the MMAs for both.  A
-// 256-row MMA reads rows 0-127 of A from rank 0's tensor memory and rows
-// 128-255 from rank 1's, tokens 0-63 of B from rank 0's shared memory and
-// 64-127 from rank 1's (the same offsets in both), and writes each CTA's
-// rows of D into its own tensor memory.
-
-GI_DEVINL uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-
-// The shared::cluster address of shared-memory offset `addr` in CTA `rank`.
-GI_DEVINL uint32_t peer_addr(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-
-// Arrive on an mbarrier of either CTA of the pair (release at cluster scope).
-GI_DEVINL void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-
-// Both CTAs of the cluster, every thread: release then acquire.
-GI_DEVINL void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-GI_DEVINL void mma_f16_2(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{ .reg .pred p; setp.ne.b32 p, %4, 0; "
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-GI_DEVINL void mma_f16_ts_2(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{ .reg .pred p; setp.ne.b32 p, %4, 0; "
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
-      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// Arrive once on `bar` (the same offset) in both CTAs of the pair when every
-// pair MMA this thread issued so far has finished.
-GI_DEVINL void mma_commit_2(uint32_t bar) {
-  const uint16_t both = 3;
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-      "h"(both)
-      : "memory");
-}
-
-// 32 lanes x 16 columns of fp32 from tensor memory, waited for in place
-// (the wait names the registers, so no use can be scheduled before it).
-GI_DEVINL void tmem_ld16(uint32_t taddr, float (&v)[16]) {
-  uint32_t r[16];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-// Shared-memory matrix descriptors (K-major).  128-byte swizzle: 8-row x
-// 128-byte atoms, 1024 bytes apart (stride byte offset), 16-byte units of a
-// row XOR-ed with the row index; the leading byte offset is unused.  No
-// swizzle: 8-row x 16-byte core matrices, `sbo` bytes between row groups and
-// `lbo` bytes between the two 8-element K halves.
-GI_DEVINL uint64_t desc_sw128(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-GI_DEVINL uint64_t desc_plain(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) |
-         ((uint64_t)1 << 46);
-}
-
 // Instruction descriptor: fp32 D, fp16 A and B, both K-major, M=128, N=128;
 // for a CTA pair M=256 (128 rows in each CTA).
 constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(kTileTok >> 3) << 17) | ((uint32_t)(kTileRows >> 4) << 24);
 constexpr uint32_t kIdesc2 = (1u << 4) | ((uint32_t)(kTileTok >> 3) << 17) | ((uint32_t)(2 * kTileRows >> 4) << 24);
-
-GI_DEVINL void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
-               : "memory");
-}
 
 GI_DEVINL uint4 ldg_nc128(const void* p) {
   uint4 r;
@@ -340,10 +149,6 @@ GI_DEVINL uint32_t h2_splat(float v) { return h2_bits(__float2half2_rn(v)); }
 GI_DEVINL float h_lo(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v & 0xFFFF))); }
 GI_DEVINL float h_hi(uint32_t v) { return __half2float(__ushort_as_half((unsigned short)(v >> 16))); }
 
-// Byte offset of 16-byte unit `u` of row `r` in a 128-byte-swizzled tile.
-GI_DEVINL uint32_t sw128_off(int r, int u) {
-  return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((u ^ (r & 7)) << 4));
-}
 // Byte offset of K half `kh` of row `r` in a 128 x 16 core-matrix tile
 // (row groups 128 bytes apart, K halves 2048 bytes apart).
 GI_DEVINL uint32_t plain_off(int r, int kh) { return (uint32_t)((r >> 3) * 128 + (r & 7) * 16 + kh * 2048); }
