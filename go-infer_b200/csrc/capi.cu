@@ -443,6 +443,7 @@ int capi_ready(CapiCtx* c) {
   if (int rc = ensure_ready()) return rc;
   c->sm_count = g.sm_count;
   c->stream = g.stream;
+  c->error = g.scratch.error;
   return 0;
 }
 

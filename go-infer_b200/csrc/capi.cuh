@@ -14,6 +14,7 @@ namespace gi {
 struct CapiCtx {
   int sm_count = 0;
   cudaStream_t stream = nullptr;  // the library's own
+  int* error = nullptr;           // set by kernels whose bounded waits give up
 };
 
 // Held for the length of an entry point.

@@ -196,6 +196,7 @@ int gi_cuda_attn_dev(const gi_cuda_kv_cache_t* cache, const gi_cuda_attn_t* attn
   a.pages_stride = (int)pages_stride;
   a.prefix_pages = prefix_pages;
   a.ws = workspace;
+  a.error = ctx.error;
   GI_CUDA_TRY(gi::attn_launch(c, a, ctx.sm_count, stream_of(ctx, stream)), "attention");
   return 0;
 }

@@ -562,6 +562,7 @@ int DecodeModel::set_kv_cache(int type) {
   a.pages = kv_pages_;
   a.pages_stride = kv.n_pages;
   a.ws = kv_ws_;
+  a.error = scratch_.error;
   kv_attn_ = a;
   return 0;
 }

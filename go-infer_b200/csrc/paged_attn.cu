@@ -23,6 +23,8 @@
 // cores cut their sums instead of rounding them and a chain of thousands of
 // positions would drift.
 //
+// Units of many rows go to wide_attn.cu.
+//
 // Bound: single tokens read the cache once (HBM).  A unit of work is (sequence, kv
 // head, 8 * MT query rows of that head's group): it reads a position once for
 // all its rows.  The units' tiles form one line that is cut into equal runs, one per
@@ -32,20 +34,22 @@
 // cp.async ring of its own and meets the others only at the end of a unit.
 #include "common.cuh"
 #include "gemv.cuh"
+#include "paged.cuh"
 #include "serve.cuh"
 
 namespace gi {
 namespace {
 
+using namespace paged;
+
 constexpr int kWarps = 4, kAttnThreads = 32 * kWarps;
 constexpr int kMergeThreads = 128;
-constexpr float kLog2e = 1.4426950408889634f;
-
-GI_DEVINL float exp2_approx(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
+// A unit's place on the line: kUnitCost tiles for its start and end (its
+// queries, the joining of the warps: 9 to 10 thousand clocks, a tile about 900
+// per CTA), then its tl tiles.  Without them the CTAs whose runs hold many
+// short sequences end last: a batch of 62 sequences of 1 to 8192 positions
+// took 135 us instead of 127.
+constexpr int kUnitCost = 8;
 
 // 16 bytes to shared memory, of which the first `bytes` (16 or 0) are read.
 GI_DEVINL void cp_async16_or_zero(uint32_t dst, const void* src, int bytes) {
@@ -56,14 +60,6 @@ GI_DEVINL void ldsm_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
                : "r"(addr));
-}
-
-// Four int8 codes as two half2 (exact): 0x6400 + (c + 128) is the half
-// 1152 + c.
-GI_DEVINL void codes_to_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  w ^= 0x80808080u;
-  lo = hsub2_u32(prmt(w, 0x64646464u, 0x4140), 0x64806480u);
-  hi = hsub2_u32(prmt(w, 0x64646464u, 0x4342), 0x64806480u);
 }
 
 // D = A(16x16 f16, row) * B(16x8 f16, col): the first of a chain.
@@ -93,39 +89,7 @@ GI_DEVINL void load_scales(uint32_t addr, uint32_t (&w)[(N + 1) / 2]) {
   }
 }
 
-// The positions and rows one launch covers: every sequence's own positions,
-// or the shared prefix as one sequence whose rows are all tokens.
-struct Pass {
-  const float* q;
-  float* out;   // rows of whole units: finished, or with ml not null the sums alone
-  float2* ml;   // [token][head] (m, sum) of whole units
-  float* parts;  // of units cut between CTAs, two slots per CTA
-  long long* line;  // [0] tiles per CTA, [1 + b] sequence b's first tile
-  const int32_t *q_start, *kv_len, *pages;
-  int pages_stride, n_seqs, n_tokens, n_heads;
-  int prefix;  // > 0: the prefix pass, of that many positions; n_seqs still counts the sequences
-  float scale;
-};
-
-struct Seq {
-  int start, fresh, len;  // first token, new tokens, positions
-};
-
 __host__ __device__ constexpr int pow2_up(int n) { return n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512; }
-
-GI_DEVINL Seq seq_of(const Pass& p, int b, int page_shift) {
-  Seq s;
-  const int first = p.prefix ? 0 : b, last = p.prefix ? p.n_seqs : b + 1;
-  s.start = max(0, min(p.q_start ? p.q_start[first] : first, p.n_tokens));
-  s.fresh = max(s.start, min(p.q_start ? p.q_start[last] : last, p.n_tokens)) - s.start;
-  s.len = p.prefix ? p.prefix : max(0, min(p.kv_len[b], p.pages_stride << page_shift));
-  return s;
-}
-
-// Positions of the sequence that new token j sees.
-GI_DEVINL int seen_by(const Pass& p, const Seq& s, int j) {
-  return p.prefix ? s.len : max(0, min(s.len, s.len - s.fresh + j + 1));
-}
 
 // HD head dim, MT groups of 8 query rows per unit, TT positions per tile, NS
 // tiles in a warp's ring.
@@ -154,90 +118,21 @@ struct Tile {
   }
 };
 
-// a / b, which fits an int; a >= 0
-GI_DEVINL int quotient(long long a, int b) {
-  return a < (1ll << 32) ? (int)((uint32_t)a / (uint32_t)b) : (int)(a / b);
-}
-
-// A unit's place on the line: kUnitCost tiles for its start and end (its
-// queries, the joining of the warps: 9 to 10 thousand clocks, a tile about 900
-// per CTA), then its tl tiles.  Without them the CTAs whose runs hold many
-// short sequences end last: a batch of 62 sequences of 1 to 8192 positions
-// took 135 us instead of 127.
-constexpr int kUnitCost = 8;
-
-// A sequence's units: rt row tiles per kv head, tl tiles per unit; places on the line.
-struct Span {
-  int rt, tl;
-  long long places;
-};
-GI_DEVINL Span span_of(const Seq& s, int group, int kv_heads, int rows, int tt) {
-  Span n;
-  n.rt = (s.fresh * group + rows - 1) / rows;  // rows: a power of two; n_tokens * n_heads fits an int
-  n.tl = max(1, (s.len + tt - 1) / tt);
-  n.places = (long long)n.rt * (n.tl + kUnitCost) * kv_heads;
-  return n;
-}
-
 template <int HD, int TYPE, int MT, int TT, int NS, int MINB>
 __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache c, Pass p) {
   using T = Tile<HD, TYPE, MT, TT, NS>;
   constexpr int NT = TT / 8, NG = TT / 16, NB = HD / 32;
   extern __shared__ __align__(128) uint8_t sm[];
-  __shared__ long long s_scan[kWarps + 1], s_first;
-  __shared__ int s_seq;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int group = p.n_heads / c.n_kv_heads;
-  const int n_seqs = p.prefix ? 1 : p.n_seqs;
-
   // ---- this CTA's run of the line of tiles ----
-  const int per = (n_seqs + kAttnThreads - 1) / kAttnThreads;
-  const int b0 = min(tid * per, n_seqs), b1 = min(b0 + per, n_seqs);
-  long long mine = 0;
   griddep_wait();
   griddep_launch_dependents();
-  for (int b = b0; b < b1; ++b)
-    mine += span_of(seq_of(p, b, c.page_shift), group, c.n_kv_heads, T::kRows, TT).places;
-  long long incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
-  }
-  if (lane == 31) s_scan[warp] = incl;
-  __syncthreads();
-  long long before = incl - mine, total = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += s_scan[w];
-    total += s_scan[w];
-  }
-  // at least one tile for every warp
-  const long long chunk = max((total + gridDim.x - 1) / (long long)gridDim.x, (long long)kWarps);
-  long long pos = (long long)blockIdx.x * chunk;
-  const long long end = min(total, pos + chunk);
-  if (blockIdx.x == 0) {
-    if (tid == 0) p.line[0] = chunk;
-    long long at = before;
-    for (int b = b0; b < b1; ++b) {
-      p.line[1 + b] = at;
-      at += span_of(seq_of(p, b, c.page_shift), group, c.n_kv_heads, T::kRows, TT).places;
-    }
-  }
-  if (pos >= end) return;
-  if (pos >= before && pos < before + mine) {
-    long long at = before;
-    int b = b0;
-    for (;; ++b) {
-      const long long n = span_of(seq_of(p, b, c.page_shift), group, c.n_kv_heads, T::kRows, TT).places;
-      if (pos < at + n) break;
-      at += n;
-    }
-    s_seq = b;
-    s_first = at;
-  }
-  __syncthreads();
-  int b = s_seq;
-  long long first = s_first;
+  Run run;
+  if (!run_of_line<kAttnThreads>(c, p, group, T::kRows, TT, kWarps, &run)) return;
+  long long pos = run.pos, first = run.first;
+  const long long end = run.end;
+  int b = run.b;
 
   uint8_t* ring = sm + warp * NS * T::kStage;
   uint8_t* sq = sm + T::kRing;
@@ -247,18 +142,18 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
 
   while (pos < end) {
     Seq s = seq_of(p, b, c.page_shift);
-    Span n = span_of(s, group, c.n_kv_heads, T::kRows, TT);
+    Span n = span_of(p, s, group, c.n_kv_heads, T::kRows, TT);
     while (pos >= first + n.places) {
       first += n.places;
       s = seq_of(p, ++b, c.page_shift);
-      n = span_of(s, group, c.n_kv_heads, T::kRows, TT);
+      n = span_of(p, s, group, c.n_kv_heads, T::kRows, TT);
     }
     const long long rel = pos - first;
-    const int unit = quotient(rel, n.tl + kUnitCost), at0 = (int)(rel - (long long)unit * (n.tl + kUnitCost));
+    const int unit = quotient(rel, n.unit), at0 = (int)(rel - (long long)unit * n.unit);
     const int h = unit / n.rt, row0 = (unit - h * n.rt) * T::kRows;
-    const int at1 = (int)min(at0 + (end - pos), (long long)(n.tl + kUnitCost));
+    const int at1 = (int)min(at0 + (end - pos), (long long)n.unit);
     pos += at1 - at0;
-    const int tile0 = max(at0 - kUnitCost, 0), count = at1 - kUnitCost - tile0;
+    const int tile0 = max(at0 - p.unit_cost, 0), count = at1 - p.unit_cost - tile0;
     if (count <= 0) break;  // the run ends before the unit's first tile
     const bool whole = count == n.tl;
     const int n_rows = min(T::kRows, s.fresh * group - row0);
@@ -578,11 +473,6 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
   }
 }
 
-// A row's sources in one pass: the whole unit's sums, or the parts of the CTAs [i0, i1] that its unit was cut into.
-struct Rows {
-  int rows, tt, part;  // of the pass's tiles
-};
-
 // Joins row (token, head) of the passes' parts, in the order of the
 // positions: the prefix, then the sequence's own.  One CTA per (token, kv head).
 // Parts come in groups of kAhead, whose loads are in flight together: a row of one
@@ -623,7 +513,7 @@ __global__ void __launch_bounds__(kMergeThreads) attn_merge_kernel(KvCache c, Pa
     const Pass& p = k ? own : pre;
     const Rows& w = k ? ro : rp;
     src[k].s = seq_of(p, k ? b : 0, c.page_shift);
-    src[k].n = span_of(src[k].s, group, c.n_kv_heads, w.rows, w.tt);
+    src[k].n = span_of(p, src[k].s, group, c.n_kv_heads, w.rows, w.tt);
     src[k].chunk = p.line[0];
     src[k].line = p.line[1 + (k ? b : 0)];
   }
@@ -640,7 +530,7 @@ __global__ void __launch_bounds__(kMergeThreads) attn_merge_kernel(KvCache c, Pa
       const Rows& w = k ? ro : rp;
       const Source& q = src[k];
       const int row = (token - q.s.start) * group + hg, r = row % w.rows;
-      const long long u1 = q.line + ((long long)h * q.n.rt + row / w.rows + 1) * (q.n.tl + kUnitCost), u0 = u1 - q.n.tl;
+      const long long u1 = q.line + ((long long)h * q.n.rt + row / w.rows + 1) * q.n.unit, u0 = u1 - q.n.tl;
       const int i0 = quotient(u0, (int)q.chunk), i1 = quotient(u1 - 1, (int)q.chunk);
       if (i0 == i1 && !p.ml) {  // finished by its CTA
         done = true;
@@ -690,7 +580,7 @@ __global__ void __launch_bounds__(kMergeThreads) attn_merge_kernel(KvCache c, Pa
 // ---- launch choices -----------------------------------------------------------
 typedef void (*TilesKernel)(KvCache, Pass);
 struct Choice {
-  TilesKernel fn;
+  TilesKernel fn;  // null: wide_attn.cu
   int smem, per_sm;
   Rows rows;
 };
@@ -712,6 +602,7 @@ Choice choose(int rows) {
 }
 
 Choice choose(const KvCache& c, int rows) {
+  if (wide_ok(c.head_dim, rows)) return {nullptr, 0, 1, wide_rows(c.head_dim)};
   const bool f16 = c.type == kTypeF16;
   switch (c.head_dim) {
     case 64: return f16 ? choose<64, kTypeF16>(rows) : choose<64, kTypeQ8_0>(rows);
@@ -760,7 +651,7 @@ int prepare() {
 int attn_prepare_device() {
   return prepare<64, kTypeF16>() || prepare<64, kTypeQ8_0>() || prepare<96, kTypeF16>() || prepare<96, kTypeQ8_0>() ||
                  prepare<128, kTypeF16>() || prepare<128, kTypeQ8_0>() || prepare<256, kTypeF16>() ||
-                 prepare<256, kTypeQ8_0>()
+                 prepare<256, kTypeQ8_0>() || wide_prepare()
              ? -5
              : 0;
 }
@@ -791,6 +682,7 @@ cudaError_t attn_launch(const KvCache& c, const Attn& a, int sm_count, cudaStrea
   own.n_tokens = a.n_tokens;
   own.n_heads = a.n_heads;
   own.scale = a.scale;
+  own.unit_cost = kUnitCost;
   Pass pre = own;
   pre.prefix = a.prefix_len;
   if (a.prefix_len) {
@@ -799,9 +691,18 @@ cudaError_t attn_launch(const KvCache& c, const Attn& a, int sm_count, cudaStrea
     pre.parts = reinterpret_cast<float*>(ws + w.parts[1]);
     pre.line = reinterpret_cast<long long*>(ws + w.line[1]);
     pre.pages = a.prefix_pages;
-    kp.fn<<<kp.per_sm * sm_count, kAttnThreads, kp.smem, s>>>(c, pre);
   }
-  ko.fn<<<ko.per_sm * sm_count, kAttnThreads, ko.smem, s>>>(c, own);
+  auto run = [&](const Choice& k, Pass& p) {
+    if (!k.fn) {
+      p.unit_cost = wide_cost();
+      return wide_launch(c, p, sm_count, a.error, s);
+    }
+    k.fn<<<k.per_sm * sm_count, kAttnThreads, k.smem, s>>>(c, p);
+    return cudaGetLastError();
+  };
+  if (a.prefix_len)
+    if (cudaError_t e = run(kp, pre)) return e;
+  if (cudaError_t e = run(ko, own)) return e;
   // the merge's CTAs come up while the tiles' drain; they wait for all of it before they read
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.n_tokens, c.n_kv_heads);
@@ -812,7 +713,6 @@ cudaError_t attn_launch(const KvCache& c, const Attn& a, int sm_count, cudaStrea
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaError_t e = cudaGetLastError()) return e;
   return cudaLaunchKernelEx(&cfg, attn_merge_kernel, c, own, ko.rows, pre, kp.rows, a.out);
 }
 

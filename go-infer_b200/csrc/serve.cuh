@@ -59,6 +59,7 @@ struct Attn {
   int pages_stride = 0;
   const int32_t* prefix_pages = nullptr;
   void* ws = nullptr;
+  int* error = nullptr;  // the library's error word
 };
 
 int attn_prepare_device();

@@ -1,0 +1,583 @@
+// wide_attn.cu -- attention over the paged cache for units of many query
+// rows (a prompt's chunk, a shared prefix under a batch): the same operator,
+// line of tiles and parts as paged_attn.cu, on the 5th-generation tensor
+// cores.
+//
+// Bound: the tensor cores.  A tile is 128 query rows x 128 positions; it
+// takes 2 x 128 x 128 x head_dim products for S = q K^T and as many for
+// P V, twice each, because q and P are split into two halves (22 bits, see
+// paged_attn.cu): about 2200 clocks at head dim 128.  Beside them run the
+// softmax (one thread per half row, no shuffles: a row is a tensor-memory
+// lane) and the conversion of the cache's values into operand tiles, by warps
+// of their own:
+//   warps 0-7    softmax: row 32 (w % 4) + lane, positions 64 (w / 4) + 0..63
+//                of the tile; also the queries, the running sums, the output
+//   warps 8-14   the tiles' groups of 16 positions in turn: K and V^T, global
+//                -> registers (a group ahead) -> shared memory, 128-byte swizzle
+//   warp 15      tcgen05.mma (one thread), tensor memory
+// (16 warps: a thread can have 128 registers)
+// K and V^T are K-major operands: V is transposed on its way through the
+// registers, where Q8_0 codes become halves in any case.  P takes the place
+// of S in tensor memory (16 columns of S become 8 of high and 8 of low
+// halves) and is the A operand of P V from there.
+// Tensor memory: S/P twice, P V twice, 128 columns each at most.
+// P V of one tile starts from zero; the running sum over tiles is a float32
+// FMA in the softmax threads' registers, so rounding does not grow with the
+// length (the tensor cores cut their sums).
+// Every wait is bounded in time; on expiry the CTA sets *error, its roles
+// leave, the products in flight are awaited (again bounded), tensor memory is freed.
+#include "common.cuh"
+#include "gemv.cuh"
+#include "paged.cuh"
+#include "serve.cuh"
+#include "tc.cuh"
+
+namespace gi {
+namespace {
+
+using namespace paged;
+using namespace tc;
+
+constexpr int kRows = 128, kTok = 128;
+constexpr int kSoftWarps = 8, kLoadWarps = 7;
+constexpr int kGroups = kTok / 16;  // of 16 positions, what a loading warp takes at a time
+constexpr int kWideThreads = 32 * (kSoftWarps + kLoadWarps + 1);
+constexpr int kWideCost = 2;  // tiles that a unit's start and end take
+constexpr int kTmem = 512;
+
+template <int HD>
+struct Wide {
+  static constexpr int kOperand = kRows * HD * 2;      // bytes of Q's high (or low) part, of K
+  static constexpr int kV = HD * kTok * 2;             // bytes of V^T: two sub-tiles of 64 positions
+  static constexpr int kQ = 0, kK = 2 * kOperand, kVt = kK + 2 * kOperand;
+  static constexpr int kEnd = kVt + 2 * kV;
+  static constexpr int kSmem = kEnd + 1024 /* alignment */ + 8192;
+  static constexpr int kPart = kRows * (HD + 2);
+  static constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kTok >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+  static constexpr uint32_t kIdescO = (1u << 4) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+};
+
+GI_DEVINL void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+// Named barrier of the softmax warps.
+GI_DEVINL void soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory"); }
+
+// A unit of this CTA's run.
+struct Unit {
+  Seq s;
+  int h, row0, n_rows, tile0, tiles, seen_first, b;
+  bool whole;
+};
+
+// The run's units in order; every role walks them by itself.
+struct Walk {
+  long long pos, end, first;
+  int b;
+  GI_DEVINL bool next(const KvCache& c, const Pass& p, int group, Unit* u) {
+    if (pos >= end) return false;
+    Seq s = seq_of(p, b, c.page_shift);
+    Span n = span_of(p, s, group, c.n_kv_heads, kRows, kTok);
+    while (pos >= first + n.places) {
+      first += n.places;
+      s = seq_of(p, ++b, c.page_shift);
+      n = span_of(p, s, group, c.n_kv_heads, kRows, kTok);
+    }
+    const long long rel = pos - first;
+    const int unit = quotient(rel, n.unit), at0 = (int)(rel - (long long)unit * n.unit);
+    const int at1 = (int)min(at0 + (end - pos), (long long)n.unit);
+    pos += at1 - at0;
+    const int tile0 = max(at0 - p.unit_cost, 0), count = at1 - p.unit_cost - tile0;
+    if (count <= 0) return false;  // the run ends before the unit's first tile
+    u->s = s;
+    u->b = b;
+    u->h = unit / n.rt;
+    u->row0 = (unit - u->h * n.rt) * kRows;
+    u->n_rows = min(kRows, s.fresh * group - u->row0);
+    u->tile0 = tile0;
+    u->whole = count == n.tl;
+    u->seen_first = seen_by(p, s, u->row0 / group);
+    const int seen_last = seen_by(p, s, (u->row0 + u->n_rows - 1) / group);
+    u->tiles = max(0, min(tile0 + count, (seen_last + kTok - 1) / kTok) - tile0);
+    return true;
+  }
+};
+
+template <int HD, int TYPE>
+__global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p, int* error) {
+  using W = Wide<HD>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023) & ~1023u;
+  uint8_t* sm = smem_raw + (base - raw);
+  float2* s_ml = reinterpret_cast<float2*>(sm + W::kEnd);          // [2][row]: a half row's statistics
+  float* s_max = reinterpret_cast<float*>(s_ml + 2 * kRows);       // [tile parity][half][row]
+  float* s_fac = s_max + 4 * kRows;                                // [row]
+  uint8_t* s_bad = reinterpret_cast<uint8_t*>(s_fac + kRows);      // [tile % 4][16-position group]
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_bad + 32);
+  volatile int* s_stop = reinterpret_cast<volatile int*>(s_tmem + 1);
+  const uint32_t bars = smem_u32(s_tmem + 4);  // 8-byte aligned: everything above is a multiple of 16 bytes
+  // barriers, [tile parity] each but the queries'
+  auto k_full = [&](int i) { return bars + 8 * i; };
+  auto v_full = [&](int i) { return bars + 8 * (2 + i); };
+  auto k_free = [&](int i) { return bars + 8 * (4 + i); };
+  auto v_free = [&](int i) { return bars + 8 * (6 + i); };
+  auto s_full = [&](int i) { return bars + 8 * (8 + i); };
+  auto p_full = [&](int i) { return bars + 8 * (10 + i); };
+  auto o_full = [&](int i) { return bars + 8 * (12 + i); };
+  auto o_free = [&](int i) { return bars + 8 * (14 + i); };
+  const uint32_t q_full = bars + 8 * 16, last = bars + 8 * 17;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = p.n_heads / c.n_kv_heads;
+
+  griddep_wait();
+  griddep_launch_dependents();
+  Run run;
+  if (!run_of_line<kWideThreads>(c, p, group, kRows, kTok, 1, &run)) return;
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(k_full(i), kGroups);
+      mbar_init(v_full(i), kGroups);
+      mbar_init(k_free(i), 1);
+      mbar_init(v_free(i), 1);
+      mbar_init(s_full(i), 1);
+      mbar_init(p_full(i), kSoftWarps);
+      mbar_init(o_full(i), 1);
+      mbar_init(o_free(i), kSoftWarps);
+    }
+    mbar_init(q_full, kSoftWarps);
+    mbar_init(last, 1);
+    fence_mbar_init();
+    *s_stop = 0;
+  }
+  if (warp == kSoftWarps + kLoadWarps) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)),
+                 "r"(kTmem)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(s_tmem);
+  auto s_col = [&](int i) { return tmem + i * kTok; };
+  auto o_col = [&](int i) { return tmem + 2 * kTok + i * 128; };
+
+  // A bounded wait by the whole warp; false ends the role.
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    int ok = 0;
+    if (lane == 0) {
+      ok = *s_stop ? 0 : wait_phase(bar, parity);
+      if (!ok && !*s_stop) {
+        *s_stop = 1;
+        atomicExch(error, 1);
+      }
+    }
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+  };
+  Walk walk = {run.pos, run.end, run.first, run.b};
+  Unit u;
+  int tile_no = 0;  // tiles of all units so far: buffer tile_no & 1, use tile_no >> 1 of it
+  auto phase = [](int i) { return (uint32_t)(i >> 1) & 1u; };
+
+  if (warp >= kSoftWarps + kLoadWarps) {
+    // ---- the products ----
+    int unit_no = 0;
+    bool ok = true;
+    auto issue_s = [&](int i) {  // S of tile i: S and P of tile i - 2 are done with (awaited below)
+      if (!wait(k_full(i & 1), phase(i))) return false;
+      if (lane == 0) {
+        tc_fence_after();
+        const uint32_t k = base + W::kK + (i & 1) * W::kOperand;
+#pragma unroll
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int d = 0; d < HD / 16; ++d) {
+            const uint32_t off = (d >> 2) * (kRows * 128) + (d & 3) * 32;
+            mma_f16(s_col(i & 1), desc_sw128(base + W::kQ + part * W::kOperand + off), desc_sw128(k + off), W::kIdescS,
+                    part | d);
+          }
+        mma_commit(s_full(i & 1));
+        mma_commit(k_free(i & 1));
+      }
+      __syncwarp();
+      return true;
+    };
+    while (ok && walk.next(c, p, group, &u)) {
+      if (!(ok = wait(q_full, unit_no & 1))) break;
+      ++unit_no;
+      for (int i = 0; i < min(u.tiles, 2) && ok; ++i) ok = issue_s(tile_no + i);
+      for (int i = 0; i < u.tiles && ok; ++i) {
+        const int n = tile_no + i;
+        ok = wait(v_full(n & 1), phase(n)) && wait(p_full(n & 1), phase(n)) && wait(o_free(n & 1), phase(n) ^ 1);
+        if (!ok) break;
+        if (lane == 0) {
+          tc_fence_after();
+          const uint32_t v = base + W::kVt + (n & 1) * W::kV;
+#pragma unroll
+          for (int t = 0; t < kTok / 16; ++t) {
+            const uint64_t b = desc_sw128(v + (t >> 2) * (HD * 128) + (t & 3) * 32);
+            mma_f16_ts(o_col(n & 1), s_col(n & 1) + 16 * t, b, W::kIdescO, t != 0);
+            mma_f16_ts(o_col(n & 1), s_col(n & 1) + 16 * t + 8, b, W::kIdescO, 1);
+          }
+          mma_commit(o_full(n & 1));
+          mma_commit(v_free(n & 1));
+        }
+        __syncwarp();
+        if (i + 2 < u.tiles) ok = wait(o_full(n & 1), phase(n)) && issue_s(n + 2);  // P is read: S may come in its place
+      }
+      tile_no += u.tiles;
+    }
+    // nothing may be in flight when the others leave
+    if (lane == 0) {
+      mma_commit(last);
+      if (!wait_phase(last, 0)) atomicExch(error, 1);
+    }
+    __syncwarp();
+  } else if (warp >= kSoftWarps) {
+    // ---- operand tiles: every 7th group of 16 positions ----
+    constexpr int kE = TYPE == kTypeF16 ? 2 : 1;
+    constexpr int kKLoads = 16 * HD * kE / 512;  // 16-byte loads of K per lane
+    constexpr int kDims = HD / 32;               // dimensions of V per lane
+    uint4 kr[kKLoads];
+    uint32_t vr[16][kDims * kE / 4 > 0 ? kDims * kE / 4 : 1];
+    uint32_t ksc = 0, vsc = 0;  // two scales of this lane's half position (Q8_0)
+    bool bad = false;
+    // head dim 64: a position has 2 scales, one word; 128: two words
+    constexpr int kScaleWords = HD / 64;
+    auto load = [&](const Unit& x, int tile, int w) {
+      const int p0 = tile * kTok + 16 * w;
+      const int32_t* pages = p.pages + (p.prefix ? 0 : (size_t)x.b * p.pages_stride);
+      const int page = p0 < x.s.len ? __ldg(pages + (p0 >> c.page_shift)) : 0;
+      bad = (unsigned)page >= (unsigned)c.n_pages;
+      const int left = bad ? 0 : x.s.len - p0;
+      const size_t at = (((size_t)(bad ? 0 : page) * c.n_kv_heads + x.h) << c.page_shift) + (p0 & (c.page_size - 1));
+      const uint8_t* k = c.k + at * HD * kE;
+      const uint8_t* v = c.v + at * HD * kE;
+#pragma unroll
+      for (int i = 0; i < kKLoads; ++i) {
+        const int ch = 32 * i + lane, r = ch / (HD * kE / 16);
+        kr[i] = r < left ? ldg_stream(k + 16 * ch) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const uint8_t* a = v + (size_t)r * HD * kE + lane * kDims * kE;
+        if (kDims * kE == 8) {
+          const uint2 x2 = r < left ? __ldg(reinterpret_cast<const uint2*>(a)) : make_uint2(0, 0);
+          vr[r][0] = x2.x;
+          vr[r][kDims * kE / 4 - 1] = x2.y;
+        } else if (kDims * kE == 4) {
+          vr[r][0] = r < left ? ldg_stream32(a) : 0u;
+        } else {  // two codes
+          vr[r][0] = r < left ? (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(a)) : 0u;
+        }
+      }
+      if (TYPE == kTypeQ8_0) {
+        const int r = lane / kScaleWords;  // lane l holds word l of the 16 positions' scales
+        const bool in = lane < 16 * kScaleWords && r < left;
+        ksc = in ? __ldg(reinterpret_cast<const uint32_t*>(c.ks + at * (HD / 32)) + lane) : 0u;
+        vsc = in ? __ldg(reinterpret_cast<const uint32_t*>(c.vs + at * (HD / 32)) + lane) : 0u;
+      }
+    };
+    // scale of position r, block b, from the lanes' words
+    auto scale_word = [&](uint32_t words, int r, int b) {
+      return __shfl_sync(0xffffffffu, words, r * kScaleWords + (b >> 1));
+    };
+    auto put_k = [&](int i, int w) {
+      const uint32_t dst = base + W::kK + (i & 1) * W::kOperand;
+#pragma unroll
+      for (int l = 0; l < kKLoads; ++l) {
+        const int ch = 32 * l + lane, per = HD * kE / 16, r = ch / per, row = 16 * w + r, x = ch - r * per;
+        if (TYPE == kTypeF16) {  // 8 values: one 16-byte unit
+          sts128(dst + (x >> 3) * (kTok * 128) + sw128_off(row, x & 7), kr[l].x, kr[l].y, kr[l].z, kr[l].w);
+        } else {  // 16 codes: two units, all of one block
+          const int b = x >> 1;
+          const uint32_t d2 = prmt(scale_word(ksc, r, b), 0u, b & 1 ? 0x3232 : 0x1010);
+          uint32_t o[8];
+          codes_to_h2(kr[l].x, o[0], o[1]);
+          codes_to_h2(kr[l].y, o[2], o[3]);
+          codes_to_h2(kr[l].z, o[4], o[5]);
+          codes_to_h2(kr[l].w, o[6], o[7]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = hmul2_u32(o[e], d2);
+          const uint32_t t = dst + (x >> 2) * (kTok * 128);
+          const int unit = 2 * (x & 3), odd = (x >> 2) & 1;  // the sub-tiles' units in turn: no two in one bank
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const bool up = (e ^ odd) != 0;
+            sts128(t + sw128_off(row, unit + up), up ? o[4] : o[0], up ? o[5] : o[1], up ? o[6] : o[2],
+                   up ? o[7] : o[3]);
+          }
+        }
+      }
+    };
+    auto put_v = [&](int i, int w) {
+      const uint32_t dst = base + W::kVt + (i & 1) * W::kV + (w >> 2) * (HD * 128);  // 64 positions per sub-tile
+      const int b = lane * kDims / 32;  // this lane's block of 32 dimensions
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // 8 positions: one 16-byte unit of each of the lane's rows
+        uint32_t o[kDims][4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int r = 8 * half + 2 * q;
+          if (TYPE == kTypeF16) {
+#pragma unroll
+            for (int e = 0; e < kDims / 2; ++e) {
+              o[2 * e][q] = prmt(vr[r][e], vr[r + 1][e], 0x5410);
+              o[2 * e + 1][q] = prmt(vr[r][e], vr[r + 1][e], 0x7632);
+            }
+          } else {
+            const uint32_t d = prmt(scale_word(vsc, r, b), scale_word(vsc, r + 1, b), b & 1 ? 0x7632 : 0x5410);
+            uint32_t x0, x1;
+            codes_to_h2(prmt(vr[r][0], vr[r + 1][0], 0x5140), x0, x1);
+            o[0][q] = hmul2_u32(x0, d);
+            o[1][q] = hmul2_u32(x1, d);
+            if (kDims == 4) {
+              codes_to_h2(prmt(vr[r][0], vr[r + 1][0], 0x7362), x0, x1);
+              o[2 % kDims][q] = hmul2_u32(x0, d);
+              o[3 % kDims][q] = hmul2_u32(x1, d);
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < kDims; ++e)
+          sts128(dst + sw128_off(lane * kDims + e, 2 * (w & 3) + half), o[e][0], o[e][1], o[e][2], o[e][3]);
+      }
+    };
+    int item = warp - kSoftWarps, at = 0;  // group item % 8 of tile item / 8; tile `at` of unit u
+    bool more = walk.next(c, p, group, &u);
+    while (more && u.tiles == 0) more = walk.next(c, p, group, &u);
+    // on to the item's tile, and its loads
+    auto fetch = [&] {
+      while (more && tile_no < item / kGroups) {
+        ++tile_no;
+        if (++at < u.tiles) continue;
+        at = 0;
+        do more = walk.next(c, p, group, &u);
+        while (more && u.tiles == 0);
+      }
+      if (more) load(u, u.tile0 + at, item % kGroups);
+    };
+    fetch();
+    while (more) {
+      const int n = tile_no, w = item % kGroups;
+      if (!wait(k_free(n & 1), phase(n) ^ 1)) break;
+      if (lane == 0) s_bad[8 * (n & 3) + w] = bad;  // read until the softmax of this tile is done
+      put_k(n, w);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(k_full(n & 1));
+      if (!wait(v_free(n & 1), phase(n) ^ 1)) break;
+      put_v(n, w);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(v_full(n & 1));
+      item += kLoadWarps;
+      fetch();
+    }
+  } else {
+    // ---- softmax ----
+    const int half = warp >> 2, r = 32 * (warp & 3) + lane;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+    constexpr int kOut = HD / 2;  // this thread's dimensions of the output
+    bool ok = true;
+    while (ok && walk.next(c, p, group, &u)) {
+      // queries: a power of two per row that puts the largest just under 2^14, then high and low halves
+      const int row = u.row0 + min(r, u.n_rows - 1);
+      const bool real = r < u.n_rows;
+      const size_t at = (size_t)(u.s.start + row / group) * p.n_heads + (size_t)u.h * group + row % group;
+      {
+        const float4* q = reinterpret_cast<const float4*>(p.q + at * HD + half * kOut);
+        float m = 0.f;
+        if (real)
+          for (int i = 0; i < kOut / 4; ++i) {
+            const float4 x = __ldg(q + i);
+            m = fmaxf(m, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+          }
+        s_max[half * kRows + r] = m;
+        soft_sync();
+        m = fmaxf(m, s_max[(half ^ 1) * kRows + r]);
+        const int ex = (int)(__float_as_uint(m) >> 23) - 127;
+        const int sh = m > 0.f ? min(13 - ex, 126) : 0;
+        const float up = exp2i(sh);
+        if (half == 0) s_fac[r] = p.scale * kLog2e * exp2i(-sh);
+#pragma unroll
+        for (int i = 0; i < kOut / 8; ++i) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float4 y = real ? __ldg(q + 2 * i + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[4 * e] = y.x * up, x[4 * e + 1] = y.y * up, x[4 * e + 2] = y.z * up, x[4 * e + 3] = y.w * up;
+          }
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            hi[e] = pack_h2(x[2 * e], x[2 * e + 1]);
+            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+            lo[e] = pack_h2(x[2 * e] - back.x, x[2 * e + 1] - back.y);
+          }
+          const int d = half * kOut + 8 * i;
+          const uint32_t off = base + W::kQ + (d >> 6) * (kRows * 128) + sw128_off(r, (d & 63) >> 3);
+          sts128(off, hi[0], hi[1], hi[2], hi[3]);
+          sts128(off + W::kOperand, lo[0], lo[1], lo[2], lo[3]);
+        }
+        fence_proxy_async_smem();
+        soft_sync();
+        if (lane == 0) mbar_arrive(q_full);
+      }
+      const float fac = s_fac[r];
+      const int seen = seen_by(p, u.s, row / group);
+      float o[kOut], m = -INFINITY, l = 0.f, alpha = 0.f;
+#pragma unroll
+      for (int i = 0; i < kOut; ++i) o[i] = 0.f;
+      // o = o alpha + P V of tile n
+      auto take = [&](int n) {
+        if (!wait(o_full(n & 1), phase(n))) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int i = 0; i < kOut; i += 16) {
+          float x[16];
+          tmem_ld16(o_col(n & 1) + lanes + half * kOut + i, x);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[i + e] = fmaf(o[i + e], alpha, x[e]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o_free(n & 1));
+        return true;
+      };
+      for (int i = 0; i < u.tiles; ++i) {
+        const int n = tile_no + i, p0 = (u.tile0 + i) * kTok + 64 * half;
+        if (!(ok = wait(s_full(n & 1), phase(n)))) break;
+        tc_fence_after();
+        const uint32_t bad = *reinterpret_cast<const volatile uint32_t*>(s_bad + 8 * (n & 3) + 4 * half);
+        const bool masked = p0 + 64 > u.seen_first || bad;
+        const uint32_t s = s_col(n & 1) + lanes + 64 * half;
+        auto scaled = [&](float x, int j) {  // j: position of the 64
+          x *= fac;
+          if (masked && (p0 + j >= seen || ((bad >> (8 * (j >> 4))) & 1))) x = -INFINITY;
+          return x;
+        };
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 64; j += 16) {
+          float x[16];
+          tmem_ld16(s + j, x);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) top = fmaxf(top, scaled(x[e], j + e));
+        }
+        s_max[((n & 1) * 2 + half) * kRows + r] = top;
+        soft_sync();
+        top = fmaxf(top, s_max[((n & 1) * 2 + (half ^ 1)) * kRows + r]);
+        const float mn = fmaxf(m, top), zero = mn == -INFINITY ? 0.f : mn;
+        const float alpha_n = exp2_approx(m - zero);
+        m = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 64; j += 16) {
+          float x[16];
+          uint32_t w[16];
+          tmem_ld16(s + j, x);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            x[e] = exp2_approx(scaled(x[e], j + e) - zero) * 16384.f;
+            sum += x[e];
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            w[e] = pack_h2(x[2 * e], x[2 * e + 1]);
+            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+            w[8 + e] = pack_h2(x[2 * e] - back.x, x[2 * e + 1] - back.y);
+          }
+          tmem_st16(s + j, w);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full(n & 1));
+        l = l * alpha_n + sum;
+        if (i > 0 && !(ok = take(n - 1))) break;
+        alpha = alpha_n;
+      }
+      if (ok && u.tiles > 0) ok = take(tile_no + u.tiles - 1);
+      tile_no += u.tiles;
+      if (!ok) break;
+
+      // ---- the row: finished, its sums, or a part ----
+      s_ml[half * kRows + r] = make_float2(m, l);
+      soft_sync();
+      const float sum = l + s_ml[(half ^ 1) * kRows + r].y;
+      float f = 1.f;
+      float* out = p.out + at * HD + half * kOut;
+      if (!u.whole) {
+        float* part = p.parts + (size_t)(2 * blockIdx.x + (u.tile0 > 0 ? 0 : 1)) * W::kPart;
+        out = part + r * HD + half * kOut;
+        if (half == 0 && real) *reinterpret_cast<float2*>(part + kRows * HD + 2 * r) = make_float2(m, sum);
+      } else if (p.ml) {
+        if (half == 0 && real) p.ml[at] = make_float2(m, sum);
+      } else {
+        f = sum > 0.f ? 1.f / sum : 0.f;
+      }
+      if (real) {
+#pragma unroll
+        for (int i = 0; i < kOut; i += 4)
+          *reinterpret_cast<float4*>(out + i) = make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
+      }
+      soft_sync();  // s_ml and s_max are read
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kSoftWarps + kLoadWarps)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmem) : "memory");
+}
+
+template <int HD, int TYPE>
+cudaError_t launch_wide(const KvCache& c, const Pass& p, int sm_count, int* error, cudaStream_t s) {
+  wide_kernel<HD, TYPE><<<sm_count, kWideThreads, Wide<HD>::kSmem, s>>>(c, p, error);
+  return cudaGetLastError();
+}
+
+template <int HD, int TYPE>
+bool prepare_wide() {
+  return cudaFuncSetAttribute(wide_kernel<HD, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Wide<HD>::kSmem) ==
+         cudaSuccess;
+}
+
+}  // namespace
+
+namespace paged {
+
+#ifndef GI_W
+#define GI_W 64
+#endif
+bool wide_ok(int head_dim, int rows) { return (head_dim == 64 || head_dim == 128) && rows >= GI_W; }
+
+Rows wide_rows(int head_dim) { return {kRows, kTok, kRows * (head_dim + 2)}; }
+
+int wide_prepare() {
+  return prepare_wide<64, kTypeF16>() && prepare_wide<64, kTypeQ8_0>() && prepare_wide<128, kTypeF16>() &&
+                 prepare_wide<128, kTypeQ8_0>()
+             ? 0
+             : -5;
+}
+
+cudaError_t wide_launch(const KvCache& c, const Pass& p, int sm_count, int* error, cudaStream_t s) {
+  const bool f16 = c.type == kTypeF16;
+  if (c.head_dim == 64)
+    return f16 ? launch_wide<64, kTypeF16>(c, p, sm_count, error, s)
+               : launch_wide<64, kTypeQ8_0>(c, p, sm_count, error, s);
+  return f16 ? launch_wide<128, kTypeF16>(c, p, sm_count, error, s)
+             : launch_wide<128, kTypeQ8_0>(c, p, sm_count, error, s);
+}
+
+int wide_cost() { return kWideCost; }
+
+}  // namespace paged
+}  // namespace gi

@@ -266,6 +266,26 @@ def test_attention_with_a_shared_prefix(kind, heads, kv, dim, prefix, lens, new)
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv,dim,lens,new,prefix", [
+    (4, 1, 128, [64], [64], 0), (4, 1, 64, [129], [33], 0), (2, 2, 128, [300, 1], [128, 1], 0),
+    (8, 1, 128, [700, 1500, 0, 40], [300, 64, 1, 40], 0), (6, 2, 64, [1000], [257], 0),
+    (4, 4, 128, [0] * 70, None, 1000), (8, 1, 64, list(range(60)), None, 513), (16, 2, 128, [30, 5], [30, 2], 2000),
+    (5, 1, 128, [9] * 33, None, 128)])
+def test_attention_of_many_rows(kind, heads, kv, dim, lens, new, prefix):
+    """Units of 128 rows: one and several tiles of 128 positions, rows and positions that do not fill them."""
+    AttnCase(sum(lens) + heads, kind, heads, kv, dim, 16, lens, new, prefix=prefix, pad=3).run()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_attention_of_many_rows_skips_pages_outside_the_cache(kind):
+    c = AttnCase(13, kind, 8, 2, 128, 16, [400, 133], [100, 20])
+    c.table[0, [0, 9, 20]], c.table[1, 8] = [-1, c.cache.n_pages, 10 ** 9], -7
+    c.d["table"].copy_(dev(c.table))
+    torch.cuda.synchronize()
+    c.run()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_attention_skips_pages_outside_the_cache(kind):
     """A page id outside the cache is never followed: its positions are not seen (also all of a sequence)."""
     c = AttnCase(3, kind, 4, 2, 128, 16, [60, 33, 16])
