@@ -66,6 +66,24 @@ GI_DEVINL void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
       : "memory");
 }
 
+// 32 lanes x 32 columns from tensor memory, waited for in place.
+GI_DEVINL void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
 // Named barrier of the softmax warps.
 GI_DEVINL void soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory"); }
 
@@ -404,8 +422,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         m = fmaxf(m, s_max[(half ^ 1) * kRows + r]);
         const int ex = (int)(__float_as_uint(m) >> 23) - 127;
         const int sh = m > 0.f ? min(13 - ex, 126) : 0;
-        const float up = exp2i(sh);
-        if (half == 0) s_fac[r] = p.scale * kLog2e * exp2i(-sh);
+        const float up = p.scale < 0.f ? -exp2i(sh) : exp2i(sh);  // the scale's sign with q: the factor on S is >= 0
+        if (half == 0) s_fac[r] = fabsf(p.scale) * kLog2e * exp2i(-sh);
 #pragma unroll
         for (int i = 0; i < kOut / 8; ++i) {
           float x[8];
@@ -440,11 +458,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         if (!wait(o_full(n & 1), phase(n))) return false;
         tc_fence_after();
 #pragma unroll
-        for (int i = 0; i < kOut; i += 16) {
-          float x[16];
-          tmem_ld16(o_col(n & 1) + lanes + half * kOut + i, x);
+        for (int i = 0; i < kOut; i += 32) {
+          float x[32];
+          tmem_ld32(o_col(n & 1) + lanes + half * kOut + i, x);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[i + e] = fmaf(o[i + e], alpha, x[e]);
+          for (int e = 0; e < 32; ++e) o[i + e] = fmaf(o[i + e], alpha, x[e]);
         }
         tc_fence_before();
         __syncwarp();
@@ -456,46 +474,70 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         if (!(ok = wait(s_full(n & 1), phase(n)))) break;
         tc_fence_after();
         const uint32_t bad = *reinterpret_cast<const volatile uint32_t*>(s_bad + 8 * (n & 3) + 4 * half);
-        const bool masked = p0 + 64 > u.seen_first || bad;
+        const bool masked = p0 + 64 > u.seen_first || bad;  // uniform in the warp
         const uint32_t s = s_col(n & 1) + lanes + 64 * half;
-        auto scaled = [&](float x, int j) {  // j: position of the 64
-          x *= fac;
-          if (masked && (p0 + j >= seen || ((bad >> (8 * (j >> 4))) & 1))) x = -INFINITY;
-          return x;
-        };
+        // positions j .. j + 15 of the 64 that this row sees
+        auto limit = [&](int j) { return (bad >> (8 * (j >> 4))) & 1 ? 0 : seen - p0 - j; };
         float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 64; j += 16) {
-          float x[16];
-          tmem_ld16(s + j, x);
+        for (int j = 0; j < 64; j += 32) {
+          float x[32];
+          tmem_ld32(s + j, x);
+          if (masked) {
+            const int l0 = limit(j), l1 = limit(j + 16);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) top = fmaxf(top, scaled(x[e], j + e));
+            for (int e = 0; e < 16; ++e) {
+              top = fmaxf(top, e < l0 ? x[e] : -INFINITY);
+              top = fmaxf(top, e < l1 ? x[16 + e] : -INFINITY);
+            }
+          } else {
+            float t2 = x[1];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              top = fmaxf(top, x[e]);
+              t2 = fmaxf(t2, x[e + 1]);
+            }
+            top = fmaxf(top, t2);
+          }
         }
         s_max[((n & 1) * 2 + half) * kRows + r] = top;
         soft_sync();
         top = fmaxf(top, s_max[((n & 1) * 2 + (half ^ 1)) * kRows + r]);
-        const float mn = fmaxf(m, top), zero = mn == -INFINITY ? 0.f : mn;
+        const float mn = top == -INFINITY ? m : fmaxf(m, top * fac), zero = mn == -INFINITY ? 0.f : mn;
         const float alpha_n = exp2_approx(m - zero);
         m = mn;
-        float sum = 0.f;
+        float sum = 0.f, sum2 = 0.f;
+        const float base14 = 14.f - zero;  // P at most 2^14
 #pragma unroll
-        for (int j = 0; j < 64; j += 16) {
-          float x[16];
-          uint32_t w[16];
-          tmem_ld16(s + j, x);
+        for (int j = 0; j < 64; j += 32) {
+          float x[32];
+          tmem_ld32(s + j, x);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            x[e] = exp2_approx(scaled(x[e], j + e) - zero) * 16384.f;
-            sum += x[e];
+          for (int e = 0; e < 32; ++e) x[e] = exp2_approx(fmaf(x[e], fac, base14));
+          if (masked) {
+            const int l0 = limit(j), l1 = limit(j + 16);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              x[e] = e < l0 ? x[e] : 0.f;
+              x[16 + e] = e < l1 ? x[16 + e] : 0.f;
+            }
           }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            w[e] = pack_h2(x[2 * e], x[2 * e + 1]);
-            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-            w[8 + e] = pack_h2(x[2 * e] - back.x, x[2 * e + 1] - back.y);
+          for (int q = 0; q < 2; ++q) {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float x0 = x[16 * q + 2 * e], x1 = x[16 * q + 2 * e + 1];
+              sum += x0;
+              sum2 += x1;
+              w[e] = pack_h2(x0, x1);
+              const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+              w[8 + e] = pack_h2(x0 - back.x, x1 - back.y);
+            }
+            tmem_st16(s + j + 16 * q, w);
           }
-          tmem_st16(s + j, w);
         }
+        sum += sum2;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
