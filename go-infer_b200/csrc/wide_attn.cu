@@ -12,8 +12,8 @@
 // of their own:
 //   warps 0-7    softmax: row 32 (w % 4) + lane, positions 64 (w / 4) + 0..63
 //                of the tile; also the queries, the running sums, the output
-//   warps 8-14   the tiles' groups of 16 positions in turn: K and V^T, global
-//                -> registers (a group ahead) -> shared memory, 128-byte swizzle
+//   warps 8-10   K, 11-14 V^T: the tiles' groups of 16 positions in turn, global
+//                -> registers (two groups ahead) -> shared memory, 128-byte swizzle
 //   warp 15      tcgen05.mma (one thread), tensor memory
 // (16 warps: a thread can have 128 registers)
 // K and V^T are K-major operands: V is transposed on its way through the
@@ -39,7 +39,7 @@ using namespace paged;
 using namespace tc;
 
 constexpr int kRows = 128, kTok = 128;
-constexpr int kSoftWarps = 8, kLoadWarps = 7;
+constexpr int kSoftWarps = 8, kKWarps = 3, kVWarps = 4, kLoadWarps = kKWarps + kVWarps;
 constexpr int kGroups = kTok / 16;  // of 16 positions, what a loading warp takes at a time
 constexpr int kWideThreads = 32 * (kSoftWarps + kLoadWarps + 1);
 constexpr int kWideCost = 2;  // tiles that a unit's start and end take
@@ -98,7 +98,7 @@ struct Unit {
 struct Walk {
   long long pos, end, first;
   int b;
-  GI_DEVINL bool next(const KvCache& c, const Pass& p, int group, Unit* u) {
+  __device__ __noinline__ bool next(const KvCache& c, const Pass& p, int group, Unit* u) {
     if (pos >= end) return false;
     Seq s = seq_of(p, b, c.page_shift);
     Span n = span_of(p, s, group, c.n_kv_heads, kRows, kTok);
@@ -127,6 +127,21 @@ struct Walk {
   }
 };
 
+// A bounded wait by the whole warp; false ends the role.
+__device__ __noinline__ bool wait_or_stop(uint32_t bar, uint32_t parity, volatile int* stop, int* error) {
+  int ok = 0;
+  if ((threadIdx.x & 31) == 0) {
+    ok = *stop ? 0 : wait_phase(bar, parity);
+    if (!ok && !*stop) {
+      *stop = 1;
+      atomicExch(error, 1);
+    }
+  }
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
+// The roles' loops share the SM's instruction cache: unrolled to the full, they ran at a
+// quarter of the speed.
 template <int HD, int TYPE>
 __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p, int* error) {
   using W = Wide<HD>;
@@ -140,6 +155,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_bad + 32);
   volatile int* s_stop = reinterpret_cast<volatile int*>(s_tmem + 1);
   const uint32_t bars = smem_u32(s_tmem + 4);  // 8-byte aligned: everything above is a multiple of 16 bytes
+  Unit* s_unit = reinterpret_cast<Unit*>(s_tmem + 4 + 2 * 18);  // the softmax warps' unit
   // barriers, [tile parity] each but the queries'
   auto k_full = [&](int i) { return bars + 8 * i; };
   auto v_full = [&](int i) { return bars + 8 * (2 + i); };
@@ -186,18 +202,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
   auto s_col = [&](int i) { return tmem + i * kTok; };
   auto o_col = [&](int i) { return tmem + 2 * kTok + i * 128; };
 
-  // A bounded wait by the whole warp; false ends the role.
-  auto wait = [&](uint32_t bar, uint32_t parity) {
-    int ok = 0;
-    if (lane == 0) {
-      ok = *s_stop ? 0 : wait_phase(bar, parity);
-      if (!ok && !*s_stop) {
-        *s_stop = 1;
-        atomicExch(error, 1);
-      }
-    }
-    return __shfl_sync(0xffffffffu, ok, 0) != 0;
-  };
+  auto wait = [&](uint32_t bar, uint32_t parity) { return wait_or_stop(bar, parity, s_stop, error); };
   Walk walk = {run.pos, run.end, run.first, run.b};
   Unit u;
   int tile_no = 0;  // tiles of all units so far: buffer tile_no & 1, use tile_no >> 1 of it
@@ -207,47 +212,57 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
     // ---- the products ----
     int unit_no = 0;
     bool ok = true;
-    auto issue_s = [&](int i) {  // S of tile i: S and P of tile i - 2 are done with (awaited below)
-      if (!wait(k_full(i & 1), phase(i))) return false;
-      if (lane == 0) {
-        tc_fence_after();
-        const uint32_t k = base + W::kK + (i & 1) * W::kOperand;
-#pragma unroll
-        for (int part = 0; part < 2; ++part)
-#pragma unroll
-          for (int d = 0; d < HD / 16; ++d) {
-            const uint32_t off = (d >> 2) * (kRows * 128) + (d & 3) * 32;
-            mma_f16(s_col(i & 1), desc_sw128(base + W::kQ + part * W::kOperand + off), desc_sw128(k + off), W::kIdescS,
-                    part | d);
-          }
-        mma_commit(s_full(i & 1));
-        mma_commit(k_free(i & 1));
-      }
-      __syncwarp();
-      return true;
-    };
     while (ok && walk.next(c, p, group, &u)) {
       if (!(ok = wait(q_full, unit_no & 1))) break;
       ++unit_no;
-      for (int i = 0; i < min(u.tiles, 2) && ok; ++i) ok = issue_s(tile_no + i);
-      for (int i = 0; i < u.tiles && ok; ++i) {
-        const int n = tile_no + i;
-        ok = wait(v_full(n & 1), phase(n)) && wait(p_full(n & 1), phase(n)) && wait(o_free(n & 1), phase(n) ^ 1);
-        if (!ok) break;
-        if (lane == 0) {
-          tc_fence_after();
-          const uint32_t v = base + W::kVt + (n & 1) * W::kV;
+      // S of tile i goes before P V of tile i - 1, which waits for the softmax
+      for (int i = 0; i <= u.tiles && ok && u.tiles; ++i) {
+        if (i < u.tiles) {
+          const int n = tile_no + i;
+          if (i >= 2) ok = wait(o_full(n & 1), phase(n - 2));  // P of tile n - 2 is read: S may come in its place
+          ok = ok && wait(k_full(n & 1), phase(n));
+          if (!ok) break;
+          if (lane == 0) {
+            tc_fence_after();
+#pragma unroll 1
+            for (int part = 0; part < 2; ++part) {
+              uint64_t q = desc_sw128(base + W::kQ + part * W::kOperand), k = desc_sw128(base + W::kK + (n & 1) * W::kOperand);
+#pragma unroll 1
+              for (int sub = 0; sub < HD / 64; ++sub) {
 #pragma unroll
-          for (int t = 0; t < kTok / 16; ++t) {
-            const uint64_t b = desc_sw128(v + (t >> 2) * (HD * 128) + (t & 3) * 32);
-            mma_f16_ts(o_col(n & 1), s_col(n & 1) + 16 * t, b, W::kIdescO, t != 0);
-            mma_f16_ts(o_col(n & 1), s_col(n & 1) + 16 * t + 8, b, W::kIdescO, 1);
+                for (int d = 0; d < 4; ++d) mma_f16(s_col(n & 1), q + 2 * d, k + 2 * d, W::kIdescS, part | sub | d);
+                q += kRows * 128 / 16;
+                k += kTok * 128 / 16;
+              }
+            }
+            mma_commit(s_full(n & 1));
+            mma_commit(k_free(n & 1));
           }
-          mma_commit(o_full(n & 1));
-          mma_commit(v_free(n & 1));
+          __syncwarp();
         }
-        __syncwarp();
-        if (i + 2 < u.tiles) ok = wait(o_full(n & 1), phase(n)) && issue_s(n + 2);  // P is read: S may come in its place
+        if (i > 0) {
+          const int n = tile_no + i - 1;
+          ok = wait(v_full(n & 1), phase(n)) && wait(p_full(n & 1), phase(n)) && wait(o_free(n & 1), phase(n) ^ 1);
+          if (!ok) break;
+          if (lane == 0) {
+            tc_fence_after();
+            uint64_t v = desc_sw128(base + W::kVt + (n & 1) * W::kV);
+            uint32_t a = s_col(n & 1);
+#pragma unroll 1
+            for (int sub = 0; sub < 2; ++sub) {
+#pragma unroll
+              for (int d = 0; d < 4; ++d) {
+                mma_f16_ts(o_col(n & 1), a + 16 * d, v + 2 * d, W::kIdescO, sub | d);
+                mma_f16_ts(o_col(n & 1), a + 16 * d + 8, v + 2 * d, W::kIdescO, 1);
+              }
+              a += 64;
+              v += HD * 128 / 16;
+            }
+            mma_commit(o_full(n & 1));
+            mma_commit(v_free(n & 1));
+          }
+          __syncwarp();
+        }
       }
       tile_no += u.tiles;
     }
@@ -258,145 +273,182 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
     }
     __syncwarp();
   } else if (warp >= kSoftWarps) {
-    // ---- operand tiles: every 7th group of 16 positions ----
+    // ---- operand tiles: a warp takes every 3rd group of K, or every 4th of V, two groups in flight ----
     constexpr int kE = TYPE == kTypeF16 ? 2 : 1;
     constexpr int kKLoads = 16 * HD * kE / 512;  // 16-byte loads of K per lane
     constexpr int kDims = HD / 32;               // dimensions of V per lane
-    uint4 kr[kKLoads];
-    uint32_t vr[16][kDims * kE / 4 > 0 ? kDims * kE / 4 : 1];
-    uint32_t ksc = 0, vsc = 0;  // two scales of this lane's half position (Q8_0)
-    bool bad = false;
-    // head dim 64: a position has 2 scales, one word; 128: two words
-    constexpr int kScaleWords = HD / 64;
-    auto load = [&](const Unit& x, int tile, int w) {
-      const int p0 = tile * kTok + 16 * w;
-      const int32_t* pages = p.pages + (p.prefix ? 0 : (size_t)x.b * p.pages_stride);
-      const int page = p0 < x.s.len ? __ldg(pages + (p0 >> c.page_shift)) : 0;
-      bad = (unsigned)page >= (unsigned)c.n_pages;
-      const int left = bad ? 0 : x.s.len - p0;
-      const size_t at = (((size_t)(bad ? 0 : page) * c.n_kv_heads + x.h) << c.page_shift) + (p0 & (c.page_size - 1));
-      const uint8_t* k = c.k + at * HD * kE;
-      const uint8_t* v = c.v + at * HD * kE;
-#pragma unroll
-      for (int i = 0; i < kKLoads; ++i) {
-        const int ch = 32 * i + lane, r = ch / (HD * kE / 16);
-        kr[i] = r < left ? ldg_stream(k + 16 * ch) : make_uint4(0, 0, 0, 0);
+    constexpr int kVWords = kDims * kE >= 4 ? kDims * kE / 4 : 1;
+    constexpr int kScaleWords = HD / 64;  // words of a position's scales
+    struct Group {
+      int tile, w;     // tile of the run, group of it
+      bool bad, real;  // no such page; whether there is such a group
+      uint32_t scales;  // Q8_0: word `lane` of the 16 positions' scales
+    };
+    const bool is_k = warp < kSoftWarps + kKWarps;
+    const int step = is_k ? kKWarps : kVWarps;
+    int item = is_k ? warp - kSoftWarps : warp - kSoftWarps - kKWarps, in_unit = 0;
+    bool more = walk.next(c, p, group, &u);
+    while (more && u.tiles == 0) more = walk.next(c, p, group, &u);
+    // The item's group: its page and scales; data goes to load().
+    const uint8_t* src = nullptr;
+    int left = 0;
+    auto next_group = [&](Group* x) {
+      while (more && tile_no < item / kGroups) {
+        ++tile_no;
+        if (++in_unit < u.tiles) continue;
+        in_unit = 0;
+        do more = walk.next(c, p, group, &u);
+        while (more && u.tiles == 0);
       }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const uint8_t* a = v + (size_t)r * HD * kE + lane * kDims * kE;
-        if (kDims * kE == 8) {
-          const uint2 x2 = r < left ? __ldg(reinterpret_cast<const uint2*>(a)) : make_uint2(0, 0);
-          vr[r][0] = x2.x;
-          vr[r][kDims * kE / 4 - 1] = x2.y;
-        } else if (kDims * kE == 4) {
-          vr[r][0] = r < left ? ldg_stream32(a) : 0u;
-        } else {  // two codes
-          vr[r][0] = r < left ? (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(a)) : 0u;
-        }
-      }
-      if (TYPE == kTypeQ8_0) {
-        const int r = lane / kScaleWords;  // lane l holds word l of the 16 positions' scales
-        const bool in = lane < 16 * kScaleWords && r < left;
-        ksc = in ? __ldg(reinterpret_cast<const uint32_t*>(c.ks + at * (HD / 32)) + lane) : 0u;
-        vsc = in ? __ldg(reinterpret_cast<const uint32_t*>(c.vs + at * (HD / 32)) + lane) : 0u;
-      }
+      x->real = more;
+      if (!more) return;
+      x->tile = tile_no;
+      x->w = item % kGroups;
+      item += step;
+      const int p0 = (u.tile0 + in_unit) * kTok + 16 * x->w;
+      const int32_t* pages = p.pages + (p.prefix ? 0 : (size_t)u.b * p.pages_stride);
+      const int page = p0 < u.s.len ? __ldg(pages + (p0 >> c.page_shift)) : 0;
+      x->bad = (unsigned)page >= (unsigned)c.n_pages;
+      left = x->bad ? 0 : u.s.len - p0;
+      const size_t at = (((size_t)(x->bad ? 0 : page) * c.n_kv_heads + u.h) << c.page_shift) + (p0 & (c.page_size - 1));
+      src = (is_k ? c.k : c.v) + at * HD * kE;
+      x->scales = 0u;
+      if (TYPE == kTypeQ8_0 && lane < 16 * kScaleWords && lane / kScaleWords < left)
+        x->scales = __ldg(reinterpret_cast<const uint32_t*>((is_k ? c.ks : c.vs) + at * (HD / 32)) + lane);
     };
     // scale of position r, block b, from the lanes' words
     auto scale_word = [&](uint32_t words, int r, int b) {
       return __shfl_sync(0xffffffffu, words, r * kScaleWords + (b >> 1));
     };
-    auto put_k = [&](int i, int w) {
-      const uint32_t dst = base + W::kK + (i & 1) * W::kOperand;
+    if (is_k) {
+      uint4 kr[2][kKLoads];
+      Group gr[2];
+      auto load = [&](uint4 (&x)[kKLoads]) {
 #pragma unroll
-      for (int l = 0; l < kKLoads; ++l) {
-        const int ch = 32 * l + lane, per = HD * kE / 16, r = ch / per, row = 16 * w + r, x = ch - r * per;
-        if (TYPE == kTypeF16) {  // 8 values: one 16-byte unit
-          sts128(dst + (x >> 3) * (kTok * 128) + sw128_off(row, x & 7), kr[l].x, kr[l].y, kr[l].z, kr[l].w);
-        } else {  // 16 codes: two units, all of one block
-          const int b = x >> 1;
-          const uint32_t d2 = prmt(scale_word(ksc, r, b), 0u, b & 1 ? 0x3232 : 0x1010);
-          uint32_t o[8];
-          codes_to_h2(kr[l].x, o[0], o[1]);
-          codes_to_h2(kr[l].y, o[2], o[3]);
-          codes_to_h2(kr[l].z, o[4], o[5]);
-          codes_to_h2(kr[l].w, o[6], o[7]);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] = hmul2_u32(o[e], d2);
-          const uint32_t t = dst + (x >> 2) * (kTok * 128);
-          const int unit = 2 * (x & 3), odd = (x >> 2) & 1;  // the sub-tiles' units in turn: no two in one bank
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const bool up = (e ^ odd) != 0;
-            sts128(t + sw128_off(row, unit + up), up ? o[4] : o[0], up ? o[5] : o[1], up ? o[6] : o[2],
-                   up ? o[7] : o[3]);
-          }
+        for (int i = 0; i < kKLoads; ++i) {
+          const int ch = 32 * i + lane;
+          x[i] = ch / (HD * kE / 16) < left ? ldg_stream(src + 16 * ch) : make_uint4(0, 0, 0, 0);
         }
-      }
-    };
-    auto put_v = [&](int i, int w) {
-      const uint32_t dst = base + W::kVt + (i & 1) * W::kV + (w >> 2) * (HD * 128);  // 64 positions per sub-tile
-      const int b = lane * kDims / 32;  // this lane's block of 32 dimensions
+      };
+      auto put = [&](const uint4 (&x)[kKLoads], const Group& y) {
+        const uint32_t dst = base + W::kK + (y.tile & 1) * W::kOperand;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {  // 8 positions: one 16-byte unit of each of the lane's rows
-        uint32_t o[kDims][4];
+        for (int l = 0; l < kKLoads; ++l) {
+          const int ch = 32 * l + lane, per = HD * kE / 16, r = ch / per, row = 16 * y.w + r, q = ch - r * per;
+          if (TYPE == kTypeF16) {  // 8 values: one 16-byte unit
+            sts128(dst + (q >> 3) * (kTok * 128) + sw128_off(row, q & 7), x[l].x, x[l].y, x[l].z, x[l].w);
+          } else {  // 16 codes: two units, all of one block
+            const int b = q >> 1;
+            const uint32_t d2 = prmt(scale_word(y.scales, r, b), 0u, b & 1 ? 0x3232 : 0x1010);
+            uint32_t o[8];
+            codes_to_h2(x[l].x, o[0], o[1]);
+            codes_to_h2(x[l].y, o[2], o[3]);
+            codes_to_h2(x[l].z, o[4], o[5]);
+            codes_to_h2(x[l].w, o[6], o[7]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int r = 8 * half + 2 * q;
-          if (TYPE == kTypeF16) {
+            for (int e = 0; e < 8; ++e) o[e] = hmul2_u32(o[e], d2);
+            const uint32_t t = dst + (q >> 2) * (kTok * 128);
+            const int unit = 2 * (q & 3), odd = (q >> 2) & 1;  // the sub-tiles' units in turn: no two in one bank
 #pragma unroll
-            for (int e = 0; e < kDims / 2; ++e) {
-              o[2 * e][q] = prmt(vr[r][e], vr[r + 1][e], 0x5410);
-              o[2 * e + 1][q] = prmt(vr[r][e], vr[r + 1][e], 0x7632);
-            }
-          } else {
-            const uint32_t d = prmt(scale_word(vsc, r, b), scale_word(vsc, r + 1, b), b & 1 ? 0x7632 : 0x5410);
-            uint32_t x0, x1;
-            codes_to_h2(prmt(vr[r][0], vr[r + 1][0], 0x5140), x0, x1);
-            o[0][q] = hmul2_u32(x0, d);
-            o[1][q] = hmul2_u32(x1, d);
-            if (kDims == 4) {
-              codes_to_h2(prmt(vr[r][0], vr[r + 1][0], 0x7362), x0, x1);
-              o[2 % kDims][q] = hmul2_u32(x0, d);
-              o[3 % kDims][q] = hmul2_u32(x1, d);
+            for (int e = 0; e < 2; ++e) {
+              const bool up = (e ^ odd) != 0;
+              sts128(t + sw128_off(row, unit + up), up ? o[4] : o[0], up ? o[5] : o[1], up ? o[6] : o[2],
+                     up ? o[7] : o[3]);
             }
           }
         }
+      };
 #pragma unroll
-        for (int e = 0; e < kDims; ++e)
-          sts128(dst + sw128_off(lane * kDims + e, 2 * (w & 3) + half), o[e][0], o[e][1], o[e][2], o[e][3]);
+      for (int i = 0; i < 2; ++i) {
+        next_group(&gr[i]);
+        if (gr[i].real) load(kr[i]);
       }
-    };
-    int item = warp - kSoftWarps, at = 0;  // group item % 8 of tile item / 8; tile `at` of unit u
-    bool more = walk.next(c, p, group, &u);
-    while (more && u.tiles == 0) more = walk.next(c, p, group, &u);
-    // on to the item's tile, and its loads
-    auto fetch = [&] {
-      while (more && tile_no < item / kGroups) {
-        ++tile_no;
-        if (++at < u.tiles) continue;
-        at = 0;
-        do more = walk.next(c, p, group, &u);
-        while (more && u.tiles == 0);
+      for (bool go = true; go;) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (!(go = go && gr[i].real)) break;
+          const int n = gr[i].tile;
+          if (!(go = wait(k_free(n & 1), phase(n) ^ 1))) break;
+          if (lane == 0) s_bad[8 * (n & 3) + gr[i].w] = gr[i].bad;  // read until the softmax of this tile is done
+          put(kr[i], gr[i]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(k_full(n & 1));
+          next_group(&gr[i]);
+          if (gr[i].real) load(kr[i]);
+        }
       }
-      if (more) load(u, u.tile0 + at, item % kGroups);
-    };
-    fetch();
-    while (more) {
-      const int n = tile_no, w = item % kGroups;
-      if (!wait(k_free(n & 1), phase(n) ^ 1)) break;
-      if (lane == 0) s_bad[8 * (n & 3) + w] = bad;  // read until the softmax of this tile is done
-      put_k(n, w);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(k_full(n & 1));
-      if (!wait(v_free(n & 1), phase(n) ^ 1)) break;
-      put_v(n, w);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(v_full(n & 1));
-      item += kLoadWarps;
-      fetch();
+    } else {
+      uint32_t vr[2][16][kVWords];
+      Group gr[2];
+      auto load = [&](uint32_t (&x)[16][kVWords]) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const uint8_t* a = src + (size_t)r * HD * kE + lane * kDims * kE;
+          if (kDims * kE == 8) {
+            const uint2 y = r < left ? __ldg(reinterpret_cast<const uint2*>(a)) : make_uint2(0, 0);
+            x[r][0] = y.x;
+            x[r][kVWords - 1] = y.y;
+          } else if (kDims * kE == 4) {
+            x[r][0] = r < left ? ldg_stream32(a) : 0u;
+          } else {  // two codes
+            x[r][0] = r < left ? (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(a)) : 0u;
+          }
+        }
+      };
+      auto put = [&](const uint32_t (&x)[16][kVWords], const Group& y) {
+        // 64 positions per sub-tile
+        const uint32_t dst = base + W::kVt + (y.tile & 1) * W::kV + (y.w >> 2) * (HD * 128);
+        const int b = lane * kDims / 32;  // this lane's block of 32 dimensions
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {  // 8 positions: one 16-byte unit of each of the lane's rows
+          uint32_t o[kDims][4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int r = 8 * half + 2 * q;
+            if (TYPE == kTypeF16) {
+#pragma unroll
+              for (int e = 0; e < kDims / 2; ++e) {
+                o[2 * e][q] = prmt(x[r][e], x[r + 1][e], 0x5410);
+                o[2 * e + 1][q] = prmt(x[r][e], x[r + 1][e], 0x7632);
+              }
+            } else {
+              const uint32_t d = prmt(scale_word(y.scales, r, b), scale_word(y.scales, r + 1, b), b & 1 ? 0x7632 : 0x5410);
+              uint32_t x0, x1;
+              codes_to_h2(prmt(x[r][0], x[r + 1][0], 0x5140), x0, x1);
+              o[0][q] = hmul2_u32(x0, d);
+              o[1][q] = hmul2_u32(x1, d);
+              if (kDims == 4) {
+                codes_to_h2(prmt(x[r][0], x[r + 1][0], 0x7362), x0, x1);
+                o[2 % kDims][q] = hmul2_u32(x0, d);
+                o[3 % kDims][q] = hmul2_u32(x1, d);
+              }
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < kDims; ++e)
+            sts128(dst + sw128_off(lane * kDims + e, 2 * (y.w & 3) + half), o[e][0], o[e][1], o[e][2], o[e][3]);
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        next_group(&gr[i]);
+        if (gr[i].real) load(vr[i]);
+      }
+      for (bool go = true; go;) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (!(go = go && gr[i].real)) break;
+          const int n = gr[i].tile;
+          if (!(go = wait(v_free(n & 1), phase(n) ^ 1))) break;
+          put(vr[i], gr[i]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v_full(n & 1));
+          next_group(&gr[i]);
+          if (gr[i].real) load(vr[i]);
+        }
+      }
     }
   } else {
     // ---- softmax ----
@@ -404,82 +456,76 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     constexpr int kOut = HD / 2;  // this thread's dimensions of the output
     bool ok = true;
-    while (ok && walk.next(c, p, group, &u)) {
-      // queries: a power of two per row that puts the largest just under 2^14, then high and low halves
-      const int row = u.row0 + min(r, u.n_rows - 1);
-      const bool real = r < u.n_rows;
-      const size_t at = (size_t)(u.s.start + row / group) * p.n_heads + (size_t)u.h * group + row % group;
+    // thread 0 walks and shows the unit: the others keep no state of the walk in registers
+    while (ok) {
+      if (tid == 0) {
+        s_unit->tiles = -1;
+        if (walk.next(c, p, group, &u)) *s_unit = u;
+      }
+      soft_sync();
+      const int tiles = s_unit->tiles;
+      if (tiles < 0) break;
+      // queries: a power of two per row that puts the largest just under 2^14, then
+      // high and low halves.  HD / 4 lanes read a row, four dimensions each.
       {
-        const float4* q = reinterpret_cast<const float4*>(p.q + at * HD + half * kOut);
-        float m = 0.f;
-        if (real)
-          for (int i = 0; i < kOut / 4; ++i) {
-            const float4 x = __ldg(q + i);
-            m = fmaxf(m, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
-          }
-        s_max[half * kRows + r] = m;
-        soft_sync();
-        m = fmaxf(m, s_max[(half ^ 1) * kRows + r]);
-        const int ex = (int)(__float_as_uint(m) >> 23) - 127;
-        const int sh = m > 0.f ? min(13 - ex, 126) : 0;
-        const float up = p.scale < 0.f ? -exp2i(sh) : exp2i(sh);  // the scale's sign with q: the factor on S is >= 0
-        if (half == 0) s_fac[r] = fabsf(p.scale) * kLog2e * exp2i(-sh);
+        const int row0 = s_unit->row0, n_rows = s_unit->n_rows;
+        const float* q0 = p.q + ((size_t)s_unit->s.start * p.n_heads + (size_t)s_unit->h * group) * HD;
+        constexpr int kPer = HD / 4, kAtOnce = 128 / HD, kBatch = 8;  // lanes per row; rows per load; loads in flight
+        const int d = 4 * (lane % kPer);
+        for (int r0 = warp * 16; r0 < warp * 16 + 16; r0 += kBatch * kAtOnce) {
+          float4 x[kBatch];
 #pragma unroll
-        for (int i = 0; i < kOut / 8; ++i) {
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float4 y = real ? __ldg(q + 2 * i + e) : make_float4(0.f, 0.f, 0.f, 0.f);
-            x[4 * e] = y.x * up, x[4 * e + 1] = y.y * up, x[4 * e + 2] = y.z * up, x[4 * e + 3] = y.w * up;
+          for (int i = 0; i < kBatch; ++i) {
+            const int qr = r0 + i * kAtOnce + lane / kPer, row_q = row0 + qr;
+            const float* q = q0 + ((size_t)(row_q / group) * p.n_heads + row_q % group) * HD;
+            x[i] = qr < n_rows ? __ldg(reinterpret_cast<const float4*>(q + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
           }
-          uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            hi[e] = pack_h2(x[2 * e], x[2 * e + 1]);
-            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-            lo[e] = pack_h2(x[2 * e] - back.x, x[2 * e + 1] - back.y);
+          for (int i = 0; i < kBatch; ++i) {
+            const int qr = r0 + i * kAtOnce + lane / kPer;
+            float m = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
+#pragma unroll
+            for (int o = kPer / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const int ex = (int)(__float_as_uint(m) >> 23) - 127;
+            const int sh = m > 0.f ? min(13 - ex, 126) : 0;
+            const float up = p.scale < 0.f ? -exp2i(sh) : exp2i(sh);  // the scale's sign with q: the factor on S is >= 0
+            if (lane % kPer == 0) s_fac[qr] = fabsf(p.scale) * kLog2e * exp2i(-sh);
+            const float y[4] = {x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up};
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              hi[e] = pack_h2(y[2 * e], y[2 * e + 1]);
+              const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+              lo[e] = pack_h2(y[2 * e] - back.x, y[2 * e + 1] - back.y);
+            }
+            const uint32_t off = base + W::kQ + (d >> 6) * (kRows * 128) + sw128_off(qr, (d & 63) >> 3) + (d & 4) * 2;
+            sts64(off, (uint64_t)hi[1] << 32 | hi[0]);
+            sts64(off + W::kOperand, (uint64_t)lo[1] << 32 | lo[0]);
           }
-          const int d = half * kOut + 8 * i;
-          const uint32_t off = base + W::kQ + (d >> 6) * (kRows * 128) + sw128_off(r, (d & 63) >> 3);
-          sts128(off, hi[0], hi[1], hi[2], hi[3]);
-          sts128(off + W::kOperand, lo[0], lo[1], lo[2], lo[3]);
         }
         fence_proxy_async_smem();
         soft_sync();
         if (lane == 0) mbar_arrive(q_full);
       }
       const float fac = s_fac[r];
-      const int seen = seen_by(p, u.s, row / group);
+      const int seen = seen_by(p, s_unit->s, (s_unit->row0 + min(r, s_unit->n_rows - 1)) / group) - s_unit->tile0 * kTok;
+      const int seen_first = s_unit->seen_first - s_unit->tile0 * kTok;  // positions from the first tile's on
       float o[kOut], m = -INFINITY, l = 0.f, alpha = 0.f;
 #pragma unroll
       for (int i = 0; i < kOut; ++i) o[i] = 0.f;
-      // o = o alpha + P V of tile n
-      auto take = [&](int n) {
-        if (!wait(o_full(n & 1), phase(n))) return false;
-        tc_fence_after();
-#pragma unroll
-        for (int i = 0; i < kOut; i += 32) {
-          float x[32];
-          tmem_ld32(o_col(n & 1) + lanes + half * kOut + i, x);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[i + e] = fmaf(o[i + e], alpha, x[e]);
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(o_free(n & 1));
-        return true;
-      };
-      for (int i = 0; i < u.tiles; ++i) {
-        const int n = tile_no + i, p0 = (u.tile0 + i) * kTok + 64 * half;
+      for (int i = 0; i <= tiles && ok && tiles; ++i) {
+        float alpha_n = 0.f;
+        if (i < tiles) {
+        const int n = tile_no + i, p0 = i * kTok + 64 * half;
         if (!(ok = wait(s_full(n & 1), phase(n)))) break;
         tc_fence_after();
         const uint32_t bad = *reinterpret_cast<const volatile uint32_t*>(s_bad + 8 * (n & 3) + 4 * half);
-        const bool masked = p0 + 64 > u.seen_first || bad;  // uniform in the warp
+        const bool masked = p0 + 64 > seen_first || bad;  // uniform in the warp
         const uint32_t s = s_col(n & 1) + lanes + 64 * half;
         // positions j .. j + 15 of the 64 that this row sees
         auto limit = [&](int j) { return (bad >> (8 * (j >> 4))) & 1 ? 0 : seen - p0 - j; };
         float top = -INFINITY;
-#pragma unroll
+#pragma unroll 1
         for (int j = 0; j < 64; j += 32) {
           float x[32];
           tmem_ld32(s + j, x);
@@ -504,38 +550,31 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         soft_sync();
         top = fmaxf(top, s_max[((n & 1) * 2 + (half ^ 1)) * kRows + r]);
         const float mn = top == -INFINITY ? m : fmaxf(m, top * fac), zero = mn == -INFINITY ? 0.f : mn;
-        const float alpha_n = exp2_approx(m - zero);
+        alpha_n = exp2_approx(m - zero);
         m = mn;
         float sum = 0.f, sum2 = 0.f;
         const float base14 = 14.f - zero;  // P at most 2^14
+#pragma unroll 1
+        for (int j = 0; j < 64; j += 16) {
+          float x[16];
+          uint32_t w[16];
+          tmem_ld16(s + j, x);
 #pragma unroll
-        for (int j = 0; j < 64; j += 32) {
-          float x[32];
-          tmem_ld32(s + j, x);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = exp2_approx(fmaf(x[e], fac, base14));
+          for (int e = 0; e < 16; ++e) x[e] = exp2_approx(fmaf(x[e], fac, base14));
           if (masked) {
-            const int l0 = limit(j), l1 = limit(j + 16);
+            const int l0 = limit(j);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              x[e] = e < l0 ? x[e] : 0.f;
-              x[16 + e] = e < l1 ? x[16 + e] : 0.f;
-            }
+            for (int e = 0; e < 16; ++e) x[e] = e < l0 ? x[e] : 0.f;
           }
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            uint32_t w[16];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float x0 = x[16 * q + 2 * e], x1 = x[16 * q + 2 * e + 1];
-              sum += x0;
-              sum2 += x1;
-              w[e] = pack_h2(x0, x1);
-              const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-              w[8 + e] = pack_h2(x0 - back.x, x1 - back.y);
-            }
-            tmem_st16(s + j + 16 * q, w);
+          for (int e = 0; e < 8; ++e) {
+            sum += x[2 * e];
+            sum2 += x[2 * e + 1];
+            w[e] = pack_h2(x[2 * e], x[2 * e + 1]);
+            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+            w[8 + e] = pack_h2(x[2 * e] - back.x, x[2 * e + 1] - back.y);
           }
+          tmem_st16(s + j, w);
         }
         sum += sum2;
         tmem_wait_st();
@@ -543,21 +582,39 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(n & 1));
         l = l * alpha_n + sum;
-        if (i > 0 && !(ok = take(n - 1))) break;
+        }
+        if (i > 0) {  // o = o alpha + P V of the tile before
+          const int n = tile_no + i - 1;
+          if (!(ok = wait(o_full(n & 1), phase(n)))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int d = 0; d < kOut; d += 32) {
+            float x[32];
+            tmem_ld32(o_col(n & 1) + lanes + half * kOut + d, x);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[d + e] = fmaf(o[d + e], alpha, x[e]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(o_free(n & 1));
+        }
         alpha = alpha_n;
       }
-      if (ok && u.tiles > 0) ok = take(tile_no + u.tiles - 1);
-      tile_no += u.tiles;
+      tile_no += tiles;
       if (!ok) break;
 
       // ---- the row: finished, its sums, or a part ----
       s_ml[half * kRows + r] = make_float2(m, l);
       soft_sync();
       const float sum = l + s_ml[(half ^ 1) * kRows + r].y;
+      const int row = s_unit->row0 + r;
+      const bool real = r < s_unit->n_rows;
+      const size_t at =
+          (size_t)(s_unit->s.start + row / group) * p.n_heads + (size_t)s_unit->h * group + row % group;
       float f = 1.f;
       float* out = p.out + at * HD + half * kOut;
-      if (!u.whole) {
-        float* part = p.parts + (size_t)(2 * blockIdx.x + (u.tile0 > 0 ? 0 : 1)) * W::kPart;
+      if (!s_unit->whole) {
+        float* part = p.parts + (size_t)(2 * blockIdx.x + (s_unit->tile0 > 0 ? 0 : 1)) * W::kPart;
         out = part + r * HD + half * kOut;
         if (half == 0 && real) *reinterpret_cast<float2*>(part + kRows * HD + 2 * r) = make_float2(m, sum);
       } else if (p.ml) {
@@ -570,7 +627,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         for (int i = 0; i < kOut; i += 4)
           *reinterpret_cast<float4*>(out + i) = make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
       }
-      soft_sync();  // s_ml and s_max are read
+      soft_sync();  // s_unit, s_ml, s_max and s_fac are read
     }
   }
   tc_fence_before();
