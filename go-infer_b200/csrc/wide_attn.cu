@@ -84,6 +84,32 @@ GI_DEVINL void tmem_ld32(uint32_t taddr, float (&v)[32]) {
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// tc.cuh's products, by the lane of a converged warp for which `mine` is 1:
+// the warp computes the operands' descriptors together, in uniform
+// registers, and only the instruction itself is predicated.  Issued from
+// inside an `if (lane == 0)` each product costs some 130 clocks of moves.
+GI_DEVINL void mma_by(uint32_t mine, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{ .reg .pred p, q; setp.ne.b32 p, %4, 0; setp.ne.b32 q, %5, 0; "
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(mine)
+      : "memory");
+}
+GI_DEVINL void mma_ts_by(uint32_t mine, uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{ .reg .pred p, q; setp.ne.b32 p, %4, 0; setp.ne.b32 q, %5, 0; "
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate), "r"(mine)
+      : "memory");
+}
+GI_DEVINL void commit_by(uint32_t mine, uint32_t bar) {
+  asm volatile(
+      "{ .reg .pred q; setp.ne.b32 q, %1, 0; "
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(bar),
+      "r"(mine)
+      : "memory");
+}
+
 // Named barrier of the softmax warps.
 GI_DEVINL void soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory"); }
 
@@ -127,17 +153,19 @@ struct Walk {
   }
 };
 
-// A bounded wait by the whole warp; false ends the role.
-__device__ __noinline__ bool wait_or_stop(uint32_t bar, uint32_t parity, volatile int* stop, int* error) {
-  int ok = 0;
-  if ((threadIdx.x & 31) == 0) {
-    ok = *stop ? 0 : wait_phase(bar, parity);
-    if (!ok && !*stop) {
+// The rest of a wait that was not over at once: bounded in time; false ends the role.
+__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* stop, int* error) {
+  const uint64_t t0 = globaltimer_ns();
+  for (;;) {
+    for (int i = 0; i < 16; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*stop) return false;
+    if (globaltimer_ns() - t0 > kWaitNs) {
       *stop = 1;
       atomicExch(error, 1);
+      return false;
     }
   }
-  return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
 // The roles' loops share the SM's instruction cache: unrolled to the full, they ran at a
@@ -158,14 +186,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
   Unit* s_unit = reinterpret_cast<Unit*>(s_tmem + 4 + 2 * 18);  // the softmax warps' unit
   // barriers, [tile parity] each but the queries'
   auto k_full = [&](int i) { return bars + 8 * i; };
-  auto v_full = [&](int i) { return bars + 8 * (2 + i); };
+  auto pv_full = [&](int i) { return bars + 8 * (2 + i); };  // V^T is there and P: P comes after the row's P V of two tiles before is taken
   auto k_free = [&](int i) { return bars + 8 * (4 + i); };
   auto v_free = [&](int i) { return bars + 8 * (6 + i); };
   auto s_full = [&](int i) { return bars + 8 * (8 + i); };
-  auto p_full = [&](int i) { return bars + 8 * (10 + i); };
-  auto o_full = [&](int i) { return bars + 8 * (12 + i); };
-  auto o_free = [&](int i) { return bars + 8 * (14 + i); };
-  const uint32_t q_full = bars + 8 * 16, last = bars + 8 * 17;
+  auto o_full = [&](int i) { return bars + 8 * (10 + i); };
+  const uint32_t q_full = bars + 8 * 12, last = bars + 8 * 13;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int group = p.n_heads / c.n_kv_heads;
 
@@ -176,13 +202,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(k_full(i), kGroups);
-      mbar_init(v_full(i), kGroups);
+      mbar_init(pv_full(i), kGroups + kSoftWarps);
       mbar_init(k_free(i), 1);
       mbar_init(v_free(i), 1);
       mbar_init(s_full(i), 1);
-      mbar_init(p_full(i), kSoftWarps);
       mbar_init(o_full(i), 1);
-      mbar_init(o_free(i), kSoftWarps);
     }
     mbar_init(q_full, kSoftWarps);
     mbar_init(last, 1);
@@ -202,7 +226,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
   auto s_col = [&](int i) { return tmem + i * kTok; };
   auto o_col = [&](int i) { return tmem + 2 * kTok + i * 128; };
 
-  auto wait = [&](uint32_t bar, uint32_t parity) { return wait_or_stop(bar, parity, s_stop, error); };
+  // By every lane of a warp, which leaves together; false ends the role.
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    const bool ok = mbar_try_wait(bar, parity) || wait_on(bar, parity, s_stop, error);
+    return __all_sync(0xffffffffu, ok) != 0;
+  };
   Walk walk = {run.pos, run.end, run.first, run.b};
   Unit u;
   int tile_no = 0;  // tiles of all units so far: buffer tile_no & 1, use tile_no >> 1 of it
@@ -212,6 +240,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
     // ---- the products ----
     int unit_no = 0;
     bool ok = true;
+    const uint32_t mine = lane == 0, tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
     while (ok && walk.next(c, p, group, &u)) {
       if (!(ok = wait(q_full, unit_no & 1))) break;
       ++unit_no;
@@ -222,46 +251,36 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
           if (i >= 2) ok = wait(o_full(n & 1), phase(n - 2));  // P of tile n - 2 is read: S may come in its place
           ok = ok && wait(k_full(n & 1), phase(n));
           if (!ok) break;
-          if (lane == 0) {
-            tc_fence_after();
-#pragma unroll 1
-            for (int part = 0; part < 2; ++part) {
-              uint64_t q = desc_sw128(base + W::kQ + part * W::kOperand), k = desc_sw128(base + W::kK + (n & 1) * W::kOperand);
-#pragma unroll 1
-              for (int sub = 0; sub < HD / 64; ++sub) {
+          tc_fence_after();
+          const int buf = __shfl_sync(0xffffffffu, n & 1, 0);
+          const uint32_t d = tmem_u + buf * kTok;
+          const uint64_t q = desc_sw128(base + W::kQ), k = desc_sw128(base + W::kK + buf * W::kOperand);
 #pragma unroll
-                for (int d = 0; d < 4; ++d) mma_f16(s_col(n & 1), q + 2 * d, k + 2 * d, W::kIdescS, part | sub | d);
-                q += kRows * 128 / 16;
-                k += kTok * 128 / 16;
-              }
+          for (int part = 0; part < 2; ++part)
+#pragma unroll
+            for (int e = 0; e < HD / 16; ++e) {
+              const int off = (e >> 2) * (kRows * 128 / 16) + (e & 3) * 2;
+              mma_by(mine, d, q + part * (W::kOperand / 16) + off, k + off, W::kIdescS, part | e);
             }
-            mma_commit(s_full(n & 1));
-            mma_commit(k_free(n & 1));
-          }
-          __syncwarp();
+          commit_by(mine, s_full(buf));
+          commit_by(mine, k_free(buf));
         }
         if (i > 0) {
           const int n = tile_no + i - 1;
-          ok = wait(v_full(n & 1), phase(n)) && wait(p_full(n & 1), phase(n)) && wait(o_free(n & 1), phase(n) ^ 1);
+          ok = wait(pv_full(n & 1), phase(n));
           if (!ok) break;
-          if (lane == 0) {
-            tc_fence_after();
-            uint64_t v = desc_sw128(base + W::kVt + (n & 1) * W::kV);
-            uint32_t a = s_col(n & 1);
-#pragma unroll 1
-            for (int sub = 0; sub < 2; ++sub) {
+          tc_fence_after();
+          const int buf = __shfl_sync(0xffffffffu, n & 1, 0);
+          const uint32_t d = tmem_u + 2 * kTok + buf * 128, a = tmem_u + buf * kTok;
+          const uint64_t v = desc_sw128(base + W::kVt + buf * W::kV);
 #pragma unroll
-              for (int d = 0; d < 4; ++d) {
-                mma_f16_ts(o_col(n & 1), a + 16 * d, v + 2 * d, W::kIdescO, sub | d);
-                mma_f16_ts(o_col(n & 1), a + 16 * d + 8, v + 2 * d, W::kIdescO, 1);
-              }
-              a += 64;
-              v += HD * 128 / 16;
-            }
-            mma_commit(o_full(n & 1));
-            mma_commit(v_free(n & 1));
+          for (int e = 0; e < kTok / 16; ++e) {
+            const uint64_t b = v + (e >> 2) * (HD * 128 / 16) + (e & 3) * 2;
+            mma_ts_by(mine, d, a + 16 * e, b, W::kIdescO, e);
+            mma_ts_by(mine, d, a + 16 * e + 8, b, W::kIdescO, 1);
           }
-          __syncwarp();
+          commit_by(mine, o_full(buf));
+          commit_by(mine, v_free(buf));
         }
       }
       tile_no += u.tiles;
@@ -279,42 +298,36 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
     constexpr int kDims = HD / 32;               // dimensions of V per lane
     constexpr int kVWords = kDims * kE >= 4 ? kDims * kE / 4 : 1;
     constexpr int kScaleWords = HD / 64;  // words of a position's scales
+    const bool is_k = warp < kSoftWarps + kKWarps;
+    const int step = is_k ? kKWarps : kVWarps, id = is_k ? warp - kSoftWarps : warp - kSoftWarps - kKWarps;
+    // The warp's groups of a unit in turn: group g of the unit's 8 * tiles is
+    // its if (8 tile_no + g) % step == id.  32 pages are looked up at a time,
+    // one per lane, so that a group's loads do not wait for its page.
     struct Group {
-      int tile, w;     // tile of the run, group of it
-      bool bad, real;  // no such page; whether there is such a group
+      const uint8_t* src;
+      int left;         // positions of the 16 that exist
+      bool bad;         // no such page
       uint32_t scales;  // Q8_0: word `lane` of the 16 positions' scales
     };
-    const bool is_k = warp < kSoftWarps + kKWarps;
-    const int step = is_k ? kKWarps : kVWarps;
-    int item = is_k ? warp - kSoftWarps : warp - kSoftWarps - kKWarps, in_unit = 0;
-    bool more = walk.next(c, p, group, &u);
-    while (more && u.tiles == 0) more = walk.next(c, p, group, &u);
-    // The item's group: its page and scales; data goes to load().
-    const uint8_t* src = nullptr;
-    int left = 0;
-    auto next_group = [&](Group* x) {
-      while (more && tile_no < item / kGroups) {
-        ++tile_no;
-        if (++in_unit < u.tiles) continue;
-        in_unit = 0;
-        do more = walk.next(c, p, group, &u);
-        while (more && u.tiles == 0);
-      }
-      x->real = more;
-      if (!more) return;
-      x->tile = tile_no;
-      x->w = item % kGroups;
-      item += step;
-      const int p0 = (u.tile0 + in_unit) * kTok + 16 * x->w;
+    int page = 0, page_of = 0;  // of group page_of + lane * step
+    auto look_up = [&](int g) {
+      page_of = g;
+      const int p0 = u.tile0 * kTok + 16 * (g + lane * step);
       const int32_t* pages = p.pages + (p.prefix ? 0 : (size_t)u.b * p.pages_stride);
-      const int page = p0 < u.s.len ? __ldg(pages + (p0 >> c.page_shift)) : 0;
-      x->bad = (unsigned)page >= (unsigned)c.n_pages;
-      left = x->bad ? 0 : u.s.len - p0;
-      const size_t at = (((size_t)(x->bad ? 0 : page) * c.n_kv_heads + u.h) << c.page_shift) + (p0 & (c.page_size - 1));
-      src = (is_k ? c.k : c.v) + at * HD * kE;
-      x->scales = 0u;
-      if (TYPE == kTypeQ8_0 && lane < 16 * kScaleWords && lane / kScaleWords < left)
-        x->scales = __ldg(reinterpret_cast<const uint32_t*>((is_k ? c.ks : c.vs) + at * (HD / 32)) + lane);
+      page = p0 < u.s.len && p0 >= 0 ? __ldg(pages + (p0 >> c.page_shift)) : 0;
+    };
+    auto group_at = [&](int g) {
+      Group x;
+      if (g >= page_of + 32 * step) look_up(g);
+      const int p0 = u.tile0 * kTok + 16 * g, pg = __shfl_sync(0xffffffffu, page, (g - page_of) / step);
+      x.bad = (unsigned)pg >= (unsigned)c.n_pages;
+      x.left = x.bad ? 0 : u.s.len - p0;
+      const size_t at = (((size_t)(x.bad ? 0 : pg) * c.n_kv_heads + u.h) << c.page_shift) + (p0 & (c.page_size - 1));
+      x.src = (is_k ? c.k : c.v) + at * HD * kE;
+      x.scales = 0u;
+      if (TYPE == kTypeQ8_0 && lane < 16 * kScaleWords && lane / kScaleWords < x.left)
+        x.scales = __ldg(reinterpret_cast<const uint32_t*>((is_k ? c.ks : c.vs) + at * (HD / 32)) + lane);
+      return x;
     };
     // scale of position r, block b, from the lanes' words
     auto scale_word = [&](uint32_t words, int r, int b) {
@@ -323,18 +336,18 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
     if (is_k) {
       uint4 kr[2][kKLoads];
       Group gr[2];
-      auto load = [&](uint4 (&x)[kKLoads]) {
+      auto load = [&](uint4 (&x)[kKLoads], const Group& y) {
 #pragma unroll
         for (int i = 0; i < kKLoads; ++i) {
           const int ch = 32 * i + lane;
-          x[i] = ch / (HD * kE / 16) < left ? ldg_stream(src + 16 * ch) : make_uint4(0, 0, 0, 0);
+          x[i] = ch / (HD * kE / 16) < y.left ? ldg_stream(y.src + 16 * ch) : make_uint4(0, 0, 0, 0);
         }
       };
-      auto put = [&](const uint4 (&x)[kKLoads], const Group& y) {
-        const uint32_t dst = base + W::kK + (y.tile & 1) * W::kOperand;
+      auto put = [&](const uint4 (&x)[kKLoads], const Group& y, int tile, int w) {
+        const uint32_t dst = base + W::kK + (tile & 1) * W::kOperand;
 #pragma unroll
         for (int l = 0; l < kKLoads; ++l) {
-          const int ch = 32 * l + lane, per = HD * kE / 16, r = ch / per, row = 16 * y.w + r, q = ch - r * per;
+          const int ch = 32 * l + lane, per = HD * kE / 16, r = ch / per, row = 16 * w + r, q = ch - r * per;
           if (TYPE == kTypeF16) {  // 8 values: one 16-byte unit
             sts128(dst + (q >> 3) * (kTok * 128) + sw128_off(row, q & 7), x[l].x, x[l].y, x[l].z, x[l].w);
           } else {  // 16 codes: two units, all of one block
@@ -358,47 +371,58 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
           }
         }
       };
+      bool go = true;
+      while (go && walk.next(c, p, group, &u)) {
+        const int n_groups = u.tiles * kGroups;
+        const int g0 = ((id - tile_no * kGroups) % step + step) % step;  // this warp's first
+        if (g0 < n_groups) look_up(g0);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        next_group(&gr[i]);
-        if (gr[i].real) load(kr[i]);
-      }
-      for (bool go = true; go;) {
+        for (int i = 0; i < 2; ++i)
+          if (g0 + i * step < n_groups) {
+            gr[i] = group_at(g0 + i * step);
+            load(kr[i], gr[i]);
+          }
+        for (int g = g0; go && g < n_groups; g += 2 * step) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (!(go = go && gr[i].real)) break;
-          const int n = gr[i].tile;
-          if (!(go = wait(k_free(n & 1), phase(n) ^ 1))) break;
-          if (lane == 0) s_bad[8 * (n & 3) + gr[i].w] = gr[i].bad;  // read until the softmax of this tile is done
-          put(kr[i], gr[i]);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(k_full(n & 1));
-          next_group(&gr[i]);
-          if (gr[i].real) load(kr[i]);
+          for (int i = 0; i < 2; ++i) {
+            const int gi = g + i * step;
+            if (gi >= n_groups) break;
+            const int n = tile_no + gi / kGroups, w = gi % kGroups;
+            if (!(go = wait(k_free(n & 1), phase(n) ^ 1))) break;
+            if (lane == 0) s_bad[8 * (n & 3) + w] = gr[i].bad;  // read until the softmax of this tile is done
+            put(kr[i], gr[i], n, w);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(k_full(n & 1));
+            if (gi + 2 * step < n_groups) {
+              gr[i] = group_at(gi + 2 * step);
+              load(kr[i], gr[i]);
+            }
+          }
         }
+        tile_no += u.tiles;
       }
     } else {
       uint32_t vr[2][16][kVWords];
       Group gr[2];
-      auto load = [&](uint32_t (&x)[16][kVWords]) {
+      auto load = [&](uint32_t (&x)[16][kVWords], const Group& y) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const uint8_t* a = src + (size_t)r * HD * kE + lane * kDims * kE;
+          const uint8_t* a = y.src + (size_t)r * HD * kE + lane * kDims * kE;
           if (kDims * kE == 8) {
-            const uint2 y = r < left ? __ldg(reinterpret_cast<const uint2*>(a)) : make_uint2(0, 0);
-            x[r][0] = y.x;
-            x[r][kVWords - 1] = y.y;
+            const uint2 z = r < y.left ? __ldg(reinterpret_cast<const uint2*>(a)) : make_uint2(0, 0);
+            x[r][0] = z.x;
+            x[r][kVWords - 1] = z.y;
           } else if (kDims * kE == 4) {
-            x[r][0] = r < left ? ldg_stream32(a) : 0u;
+            x[r][0] = r < y.left ? ldg_stream32(a) : 0u;
           } else {  // two codes
-            x[r][0] = r < left ? (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(a)) : 0u;
+            x[r][0] = r < y.left ? (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(a)) : 0u;
           }
         }
       };
-      auto put = [&](const uint32_t (&x)[16][kVWords], const Group& y) {
+      auto put = [&](const uint32_t (&x)[16][kVWords], const Group& y, int tile, int w) {
         // 64 positions per sub-tile
-        const uint32_t dst = base + W::kVt + (y.tile & 1) * W::kV + (y.w >> 2) * (HD * 128);
+        const uint32_t dst = base + W::kVt + (tile & 1) * W::kV + (w >> 2) * (HD * 128);
         const int b = lane * kDims / 32;  // this lane's block of 32 dimensions
 #pragma unroll
         for (int half = 0; half < 2; ++half) {  // 8 positions: one 16-byte unit of each of the lane's rows
@@ -427,27 +451,38 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
           }
 #pragma unroll
           for (int e = 0; e < kDims; ++e)
-            sts128(dst + sw128_off(lane * kDims + e, 2 * (y.w & 3) + half), o[e][0], o[e][1], o[e][2], o[e][3]);
+            sts128(dst + sw128_off(lane * kDims + e, 2 * (w & 3) + half), o[e][0], o[e][1], o[e][2], o[e][3]);
         }
       };
+      bool go = true;
+      while (go && walk.next(c, p, group, &u)) {
+        const int n_groups = u.tiles * kGroups;
+        const int g0 = ((id - tile_no * kGroups) % step + step) % step;  // this warp's first
+        if (g0 < n_groups) look_up(g0);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        next_group(&gr[i]);
-        if (gr[i].real) load(vr[i]);
-      }
-      for (bool go = true; go;) {
+        for (int i = 0; i < 2; ++i)
+          if (g0 + i * step < n_groups) {
+            gr[i] = group_at(g0 + i * step);
+            load(vr[i], gr[i]);
+          }
+        for (int g = g0; go && g < n_groups; g += 2 * step) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (!(go = go && gr[i].real)) break;
-          const int n = gr[i].tile;
-          if (!(go = wait(v_free(n & 1), phase(n) ^ 1))) break;
-          put(vr[i], gr[i]);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(v_full(n & 1));
-          next_group(&gr[i]);
-          if (gr[i].real) load(vr[i]);
+          for (int i = 0; i < 2; ++i) {
+            const int gi = g + i * step;
+            if (gi >= n_groups) break;
+            const int n = tile_no + gi / kGroups, w = gi % kGroups;
+            if (!(go = wait(v_free(n & 1), phase(n) ^ 1))) break;
+            put(vr[i], gr[i], n, w);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(pv_full(n & 1));
+            if (gi + 2 * step < n_groups) {
+              gr[i] = group_at(gi + 2 * step);
+              load(vr[i], gr[i]);
+            }
+          }
         }
+        tile_no += u.tiles;
       }
     }
   } else {
@@ -580,7 +615,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full(n & 1));
+        if (lane == 0) mbar_arrive(pv_full(n & 1));
         l = l * alpha_n + sum;
         }
         if (i > 0) {  // o = o alpha + P V of the tile before
@@ -595,8 +630,6 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
             for (int e = 0; e < 32; ++e) o[d + e] = fmaf(o[d + e], alpha, x[e]);
           }
           tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(o_free(n & 1));
         }
         alpha = alpha_n;
       }
