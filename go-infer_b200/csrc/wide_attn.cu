@@ -334,8 +334,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
       return __shfl_sync(0xffffffffu, words, r * kScaleWords + (b >> 1));
     };
     if (is_k) {
-      uint4 kr[2][kKLoads];
-      Group gr[2];
+      uint4 kr[kKLoads], kn[kKLoads];  // the group at hand, the next
+      Group gr, gn;
       auto load = [&](uint4 (&x)[kKLoads], const Group& y) {
 #pragma unroll
         for (int i = 0; i < kKLoads; ++i) {
@@ -376,35 +376,36 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         const int n_groups = u.tiles * kGroups;
         const int g0 = ((id - tile_no * kGroups) % step + step) % step;  // this warp's first
         if (g0 < n_groups) look_up(g0);
+        if (g0 < n_groups) {
+          gr = group_at(g0);
+          load(kr, gr);
+        }
+        if (g0 + step < n_groups) {
+          gn = group_at(g0 + step);
+          load(kn, gn);
+        }
+#pragma unroll 1
+        for (int g = g0; g < n_groups; g += step) {
+          const int n = tile_no + g / kGroups, w = g % kGroups;
+          if (!(go = wait(k_free(n & 1), phase(n) ^ 1))) break;
+          if (lane == 0) s_bad[8 * (n & 3) + w] = gr.bad;  // read until the softmax of this tile is done
+          put(kr, gr, n, w);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(k_full(n & 1));
+          gr = gn;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (g0 + i * step < n_groups) {
-            gr[i] = group_at(g0 + i * step);
-            load(kr[i], gr[i]);
-          }
-        for (int g = g0; go && g < n_groups; g += 2 * step) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int gi = g + i * step;
-            if (gi >= n_groups) break;
-            const int n = tile_no + gi / kGroups, w = gi % kGroups;
-            if (!(go = wait(k_free(n & 1), phase(n) ^ 1))) break;
-            if (lane == 0) s_bad[8 * (n & 3) + w] = gr[i].bad;  // read until the softmax of this tile is done
-            put(kr[i], gr[i], n, w);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(k_full(n & 1));
-            if (gi + 2 * step < n_groups) {
-              gr[i] = group_at(gi + 2 * step);
-              load(kr[i], gr[i]);
-            }
+          for (int i = 0; i < kKLoads; ++i) kr[i] = kn[i];
+          if (g + 2 * step < n_groups) {
+            gn = group_at(g + 2 * step);
+            load(kn, gn);
           }
         }
         tile_no += u.tiles;
       }
     } else {
-      uint32_t vr[2][16][kVWords];
-      Group gr[2];
+      uint32_t vr[16][kVWords], vn[16][kVWords];
+      Group gr, gn;
       auto load = [&](uint32_t (&x)[16][kVWords], const Group& y) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -459,27 +460,30 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         const int n_groups = u.tiles * kGroups;
         const int g0 = ((id - tile_no * kGroups) % step + step) % step;  // this warp's first
         if (g0 < n_groups) look_up(g0);
+        if (g0 < n_groups) {
+          gr = group_at(g0);
+          load(vr, gr);
+        }
+        if (g0 + step < n_groups) {
+          gn = group_at(g0 + step);
+          load(vn, gn);
+        }
+#pragma unroll 1
+        for (int g = g0; g < n_groups; g += step) {
+          const int n = tile_no + g / kGroups, w = g % kGroups;
+          if (!(go = wait(v_free(n & 1), phase(n) ^ 1))) break;
+          put(vr, gr, n, w);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(pv_full(n & 1));
+          gr = gn;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (g0 + i * step < n_groups) {
-            gr[i] = group_at(g0 + i * step);
-            load(vr[i], gr[i]);
-          }
-        for (int g = g0; go && g < n_groups; g += 2 * step) {
+          for (int r = 0; r < 16; ++r)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int gi = g + i * step;
-            if (gi >= n_groups) break;
-            const int n = tile_no + gi / kGroups, w = gi % kGroups;
-            if (!(go = wait(v_free(n & 1), phase(n) ^ 1))) break;
-            put(vr[i], gr[i], n, w);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(pv_full(n & 1));
-            if (gi + 2 * step < n_groups) {
-              gr[i] = group_at(gi + 2 * step);
-              load(vr[i], gr[i]);
-            }
+            for (int i = 0; i < kVWords; ++i) vr[r][i] = vn[r][i];
+          if (g + 2 * step < n_groups) {
+            gn = group_at(g + 2 * step);
+            load(vn, gn);
           }
         }
         tile_no += u.tiles;
@@ -507,12 +511,15 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         const float* q0 = p.q + ((size_t)s_unit->s.start * p.n_heads + (size_t)s_unit->h * group) * HD;
         constexpr int kPer = HD / 4, kAtOnce = 128 / HD, kBatch = 8;  // lanes per row; rows per load; loads in flight
         const int d = 4 * (lane % kPer);
+        // the warp's 16 rows, one per lane: their places in q
+        const int my = row0 + warp * 16 + (lane & 15);
+        const int place = (my / group) * p.n_heads + my % group;  // n_tokens * n_heads fits an int
         for (int r0 = warp * 16; r0 < warp * 16 + 16; r0 += kBatch * kAtOnce) {
           float4 x[kBatch];
 #pragma unroll
           for (int i = 0; i < kBatch; ++i) {
-            const int qr = r0 + i * kAtOnce + lane / kPer, row_q = row0 + qr;
-            const float* q = q0 + ((size_t)(row_q / group) * p.n_heads + row_q % group) * HD;
+            const int qr = r0 + i * kAtOnce + lane / kPer;
+            const float* q = q0 + (size_t)__shfl_sync(0xffffffffu, place, qr & 15) * HD;
             x[i] = qr < n_rows ? __ldg(reinterpret_cast<const float4*>(q + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
           }
 #pragma unroll
@@ -568,18 +575,17 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
             const int l0 = limit(j), l1 = limit(j + 16);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              top = fmaxf(top, e < l0 ? x[e] : -INFINITY);
-              top = fmaxf(top, e < l1 ? x[16 + e] : -INFINITY);
+              x[e] = e < l0 ? x[e] : -INFINITY;
+              x[16 + e] = e < l1 ? x[16 + e] : -INFINITY;
             }
-          } else {
-            float t2 = x[1];
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              top = fmaxf(top, x[e]);
-              t2 = fmaxf(t2, x[e + 1]);
-            }
-            top = fmaxf(top, t2);
           }
+          float t2 = x[1];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            top = fmaxf(top, x[e]);
+            t2 = fmaxf(t2, x[e + 1]);
+          }
+          top = fmaxf(top, t2);
         }
         s_max[((n & 1) * 2 + half) * kRows + r] = top;
         soft_sync();
