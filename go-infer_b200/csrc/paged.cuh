@@ -38,6 +38,7 @@ struct Pass {
   int prefix;  // > 0: the prefix pass, of that many positions; n_seqs still counts the sequences
   float scale;
   int unit_cost;  // see span_of
+  int beside;     // launched to run beside the kernel before it, whose results it does not read
 };
 
 struct Seq {

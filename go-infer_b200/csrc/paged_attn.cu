@@ -126,10 +126,13 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int group = p.n_heads / c.n_kv_heads;
   // ---- this CTA's run of the line of tiles ----
-  griddep_wait();
+  if (!p.beside) griddep_wait();
   griddep_launch_dependents();
   Run run;
-  if (!run_of_line<kAttnThreads>(c, p, group, T::kRows, TT, kWarps, &run)) return;
+  if (!run_of_line<kAttnThreads>(c, p, group, T::kRows, TT, kWarps, &run)) {
+    if (p.beside) griddep_wait();  // its end is also the end of the kernel it ran beside
+    return;
+  }
   long long pos = run.pos, first = run.first;
   const long long end = run.end;
   int b = run.b;
@@ -471,6 +474,7 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
     }
     __syncthreads();
   }
+  if (p.beside) griddep_wait();
 }
 
 // Joins row (token, head) of the passes' parts, in the order of the
@@ -612,6 +616,23 @@ Choice choose(const KvCache& c, int rows) {
   }
 }
 
+// A launch whose CTAs may come up before the kernel in front of it has ended (`early`; they wait where they
+// read its results), or after it.
+template <typename... K, typename... A>
+cudaError_t launch_after(dim3 grid, int threads, int smem, cudaStream_t s, bool early, void (*k)(K...), A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, k, static_cast<K>(args)...);
+}
+
 // The workspace: each pass's line and parts, and with a prefix the whole units' sums of both.
 struct Layout {
   size_t line[2], parts[2], ml[2], sums, bytes;
@@ -697,23 +718,16 @@ cudaError_t attn_launch(const KvCache& c, const Attn& a, int sm_count, cudaStrea
       p.unit_cost = wide_cost();
       return wide_launch(c, p, sm_count, a.error, s);
     }
-    k.fn<<<k.per_sm * sm_count, kAttnThreads, k.smem, s>>>(c, p);
-    return cudaGetLastError();
+    return launch_after(k.per_sm * sm_count, kAttnThreads, k.smem, s, p.beside != 0, k.fn, c, p);
   };
+  // The own positions' kernel needs nothing of the prefix's: it fills the SMs as that one's CTAs end.
+  own.beside = a.prefix_len && ko.fn;
   if (a.prefix_len)
     if (cudaError_t e = run(kp, pre)) return e;
   if (cudaError_t e = run(ko, own)) return e;
   // the merge's CTAs come up while the tiles' drain; they wait for all of it before they read
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.n_tokens, c.n_kv_heads);
-  cfg.blockDim = dim3(kMergeThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attn_merge_kernel, c, own, ko.rows, pre, kp.rows, a.out);
+  return launch_after(dim3(a.n_tokens, c.n_kv_heads), kMergeThreads, 0, s, true, attn_merge_kernel, c, own, ko.rows, pre,
+                      kp.rows, a.out);
 }
 
 }  // namespace gi

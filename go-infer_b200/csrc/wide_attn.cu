@@ -12,8 +12,8 @@
 // of their own:
 //   warps 0-7    softmax: row 32 (w % 4) + lane, positions 64 (w / 4) + 0..63
 //                of the tile; also the queries, the running sums, the output
-//   warps 8-10   K, 11-14 V^T: the tiles' groups of 16 positions in turn, global
-//                -> registers (two groups ahead) -> shared memory, 128-byte swizzle
+//   warps 8-11   K, 12-14 V^T: the tiles' groups of 16 positions in turn, global
+//                -> registers (a group ahead) -> shared memory, 128-byte swizzle
 //   warp 15      tcgen05.mma (one thread), tensor memory
 // (16 warps: a thread can have 128 registers)
 // K and V^T are K-major operands: V is transposed on its way through the
@@ -39,7 +39,7 @@ using namespace paged;
 using namespace tc;
 
 constexpr int kRows = 128, kTok = 128;
-constexpr int kSoftWarps = 8, kKWarps = 3, kVWarps = 4, kLoadWarps = kKWarps + kVWarps;
+constexpr int kSoftWarps = 8, kKWarps = 4, kVWarps = 3, kLoadWarps = kKWarps + kVWarps;
 constexpr int kGroups = kTok / 16;  // of 16 positions, what a loading warp takes at a time
 constexpr int kWideThreads = 32 * (kSoftWarps + kLoadWarps + 1);
 constexpr int kWideCost = 2;  // tiles that a unit's start and end take
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
     }
     __syncwarp();
   } else if (warp >= kSoftWarps) {
-    // ---- operand tiles: a warp takes every 3rd group of K, or every 4th of V, two groups in flight ----
+    // ---- operand tiles: a warp takes every 4th group of K, or every 3rd of V, the next group's loads in flight ----
     constexpr int kE = TYPE == kTypeF16 ? 2 : 1;
     constexpr int kKLoads = 16 * HD * kE / 512;  // 16-byte loads of K per lane
     constexpr int kDims = HD / 32;               // dimensions of V per lane
@@ -361,13 +361,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = hmul2_u32(o[e], d2);
             const uint32_t t = dst + (q >> 2) * (kTok * 128);
-            const int unit = 2 * (q & 3), odd = (q >> 2) & 1;  // the sub-tiles' units in turn: no two in one bank
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const bool up = (e ^ odd) != 0;
-              sts128(t + sw128_off(row, unit + up), up ? o[4] : o[0], up ? o[5] : o[1], up ? o[6] : o[2],
-                     up ? o[7] : o[3]);
-            }
+            const int unit = 2 * (q & 3);
+            sts128(t + sw128_off(row, unit), o[0], o[1], o[2], o[3]);
+            sts128(t + sw128_off(row, unit + 1), o[4], o[5], o[6], o[7]);
           }
         }
       };
