@@ -256,11 +256,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
           const uint32_t d = tmem_u + buf * kTok;
           const uint64_t q = desc_sw128(base + W::kQ), k = desc_sw128(base + W::kK + buf * W::kOperand);
 #pragma unroll
-          for (int part = 0; part < 2; ++part)
+          for (int part = 0; part < 2; ++part)  // the low halves first: each step cuts the sum, and theirs is small
 #pragma unroll
             for (int e = 0; e < HD / 16; ++e) {
               const int off = (e >> 2) * (kRows * 128 / 16) + (e & 3) * 2;
-              mma_by(mine, d, q + part * (W::kOperand / 16) + off, k + off, W::kIdescS, part | e);
+              mma_by(mine, d, q + (1 - part) * (W::kOperand / 16) + off, k + off, W::kIdescS, part | e);
             }
           commit_by(mine, s_full(buf));
           commit_by(mine, k_free(buf));
@@ -274,11 +274,11 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
           const uint32_t d = tmem_u + 2 * kTok + buf * 128, a = tmem_u + buf * kTok;
           const uint64_t v = desc_sw128(base + W::kVt + buf * W::kV);
 #pragma unroll
-          for (int e = 0; e < kTok / 16; ++e) {
-            const uint64_t b = v + (e >> 2) * (HD * 128 / 16) + (e & 3) * 2;
-            mma_ts_by(mine, d, a + 16 * e, b, W::kIdescO, e);
-            mma_ts_by(mine, d, a + 16 * e + 8, b, W::kIdescO, 1);
-          }
+          for (int part = 0; part < 2; ++part)
+#pragma unroll
+            for (int e = 0; e < kTok / 16; ++e)
+              mma_ts_by(mine, d, a + 16 * e + 8 * (1 - part), v + (e >> 2) * (HD * 128 / 16) + (e & 3) * 2, W::kIdescO,
+                        part | e);
           commit_by(mine, o_full(buf));
           commit_by(mine, v_free(buf));
         }
@@ -590,14 +590,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         alpha_n = exp2_approx(m - zero);
         m = mn;
         float sum = 0.f, sum2 = 0.f;
-        const float base14 = 14.f - zero;  // P at most 2^14
 #pragma unroll 1
         for (int j = 0; j < 64; j += 16) {
           float x[16];
           uint32_t w[16];
           tmem_ld16(s + j, x);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = exp2_approx(fmaf(x[e], fac, base14));
+          for (int e = 0; e < 16; ++e) x[e] = exp2_approx(fmaf(x[e], fac, -zero)) * 16384.f;  // not 2^14 in the exponent: 24 bits there lose 2^-21
           if (masked) {
             const int l0 = limit(j);
 #pragma unroll
