@@ -236,8 +236,12 @@ int gi_cuda_model_set_kv_cache(gi_cuda_model_t model, int type) {
   gi::ModelHandle* h = static_cast<gi::ModelHandle*>(model);
   GI_CUDA_TRY(cudaStreamSynchronize(ctx.stream), "cache type");
   h->m.drop_graphs();  // captured with the other cache
-  const int rc = h->m.set_kv_cache(type);
-  if (rc == -2) return fail(rc, "the persistent layers need the float32 cache");
+  int rc = -5;
+  try {
+    rc = h->m.set_kv_cache(type);
+  } catch (...) {  // no memory for the tables on the host
+  }
+  if (rc == -2) return fail(rc, "the persistent layers and tensor parallelism need the float32 cache");
   if (rc == -4) return fail(rc, "F16 and Q8_0 caches take head dims 64, 96, 128 and 256");
   if (rc) return fail(rc, "cache buffers", cudaGetLastError());
   h->m.reset_cache(ctx.stream);
@@ -267,7 +271,12 @@ int gi_cuda_model_generate_sampled(gi_cuda_model_t model, const int32_t* tokens,
     if (rc == -2) return fail(rc, "sampling under tensor parallelism");
     return rc ? fail(rc, "sampling buffers", cudaGetLastError()) : 0;
   };
-  const int rc = gi::model_generate(h, tokens, n_tokens, start_pos, n_gen, begin, out_tokens, out_logits, decode_ms);
+  int rc = 0;
+  try {
+    rc = gi::model_generate(h, tokens, n_tokens, start_pos, n_gen, begin, out_tokens, out_logits, decode_ms);
+  } catch (...) {
+    rc = fail(-5, "no host memory for the uniform numbers");
+  }
   h->m.stop_sampling();
   return rc;
 }

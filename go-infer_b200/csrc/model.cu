@@ -486,7 +486,7 @@ int DecodeModel::set_persistent(bool on) {
 
 int DecodeModel::set_kv_cache(int type) {
   if (type == kv_type_) return 0;
-  if ((type != kTypeF32 && type != kTypeF16 && type != kTypeQ8_0) || plan_) return -2;
+  if ((type != kTypeF32 && type != kTypeF16 && type != kTypeQ8_0) || plan_ || cfg_.tp_world > 1) return -2;
   const ModelCfg& c = cfg_;
   if (type != kTypeF32 && !attn_head_dim_ok(c.head_dim)) return -4;
   size_t t = 0;

@@ -83,8 +83,8 @@ class DecodeModel {
   bool persistent() const { return plan_ != nullptr; }
   // Cache type of each layer's K and V: kTypeF32 (the rolling float32 cache
   // of attn.cuh, the default), kTypeF16 or kTypeQ8_0 (kvcache.cu, with
-  // paged_attn.cu reading it).  Empties the cache.  -2 for another type or
-  // while the persistent kernel is on, -4 for a head dim that paged_attn.cu
+  // paged_attn.cu reading it).  Empties the cache.  -2 for another type, while
+  // the persistent kernel is on or under tensor parallelism (never run there), -4 for a head dim that paged_attn.cu
   // does not have, -5 on a CUDA error (the old cache then stays).
   int set_kv_cache(int type);
   int kv_type() const { return kv_type_; }

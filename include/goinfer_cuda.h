@@ -440,8 +440,8 @@ int gi_cuda_kv_read_dev(const gi_cuda_kv_cache_t* cache, float* k, float* v, con
 
 /* What an attention call's kernels and workspace are chosen by: n_heads query
  * heads (a multiple of the cache's n_kv_heads); at most max_tokens tokens and
- * as many sequences in a call, and max_q_len tokens of one sequence (choices follow max_q_len, results do not
- * depend on it); prefix_len positions that every sequence sees before its
+ * as many sequences in a call, and max_q_len tokens of one sequence (the kernels are chosen by max_q_len; a longer
+ * sequence is answered all the same, only slower); prefix_len positions that every sequence sees before its
  * own; scale on q.k. */
 typedef struct {
   uint32_t n_heads, max_tokens, max_q_len, prefix_len;
@@ -460,8 +460,9 @@ int64_t gi_cuda_attn_workspace(const gi_cuda_kv_cache_t* cache, const gi_cuda_at
  * of its kv_len[b] positions, which lie in pages[b * pages_stride ...] and are
  * in the cache already.  A token sees the prefix (prefix_pages; NULL when
  * prefix_len is 0) and its sequence's positions up to its own.  A row that sees
- * nothing is 0; rows behind the last sequence are left as they are.  Positions
- * that a sequence does not have are not read, whatever their pages hold. */
+ * nothing is 0; rows of no sequence are left as they are.  Positions that a
+ * sequence does not have are not read, whatever their pages hold.  out and the
+ * workspace may not overlap q or the cache. */
 int gi_cuda_attn_dev(const gi_cuda_kv_cache_t* cache, const gi_cuda_attn_t* attn, float* out, const float* q,
                      uint32_t n_seqs, uint32_t n_tokens, const int32_t* q_start, const int32_t* kv_len,
                      const int32_t* pages, uint32_t pages_stride, const int32_t* prefix_pages, void* workspace,
@@ -471,8 +472,8 @@ int gi_cuda_attn_dev(const gi_cuda_kv_cache_t* cache, const gi_cuda_attn_t* attn
  * rolling float32 cache), GI_TYPE_F16 or GI_TYPE_Q8_0 (half, or a quarter
  * and a sixteenth, of its size), written and read by the calls above
  * (kvcache.go's cache types).  Changing the type empties the cache; the step
- * is captured again at the next generate.  -2 for another type or while the
- * persistent layers are on, -4 for a head dim that gi_cuda_attn_dev does not
+ * is captured again at the next generate.  -2 for another type, while the
+ * persistent layers are on, or under tensor parallelism; -4 for a head dim that gi_cuda_attn_dev does not
  * take. */
 int gi_cuda_model_set_kv_cache(gi_cuda_model_t model, int type);
 

@@ -89,7 +89,7 @@ def attention(cache, q, q_start, kv_len, pages, scale, prefix_pages=(), prefix_l
                 w = np.exp(s - s.max())
                 w /= w.sum()
                 out[j, h] = w @ y
-                norm = np.linalg.norm(q[j, h]) * np.linalg.norm(x, axis=1).max() * scale
+                norm = np.linalg.norm(q[j, h]) * np.linalg.norm(x, axis=1).max() * abs(scale)  # a size: whatever the scale's sign
                 off = 2 * (norm * (2.0 ** -22 + dim * 2.0 ** -24) + (abs(s).max() + 1) * 2.0 ** -23)
                 bound[j, h] = (off + 64 * 2.0 ** -24) * np.abs(y).max()
     return out, bound

@@ -166,7 +166,7 @@ def test_read(kind, n, kv, dim, page):
 class AttnCase:
     """A batch with its pages anywhere in the cache, and one poisoned page that no table entry in use names."""
 
-    def __init__(self, seed, kind, heads, kv, dim, page, lens, new=None, prefix=0, pad=0):
+    def __init__(self, seed, kind, heads, kv, dim, page, lens, new=None, prefix=0, pad=0, before=0, scale=None, hint=0):
         rng = np.random.default_rng(seed)
         self.new = new or [1] * len(lens)
         self.lens, self.prefix, self.page, self.kind = list(lens), prefix, page, kind
@@ -189,15 +189,15 @@ class AttnCase:
         if prefix % page:
             for x in ((self.cache.k, self.cache.v) if kind == G.TYPE_F16 else (self.cache.ks, self.cache.vs)):
                 x[self.prefix_pages[-1], :, prefix % page:] = np.nan
-        self.start = np.concatenate(([0], np.cumsum(self.new))).astype(np.int32)
+        self.start = (before + np.concatenate(([0], np.cumsum(self.new)))).astype(np.int32)
         self.tokens = int(self.start[-1]) + pad
         self.q = rng.normal(size=(self.tokens, heads, dim)).astype(np.float32)
-        self.scale = dim ** -0.5
+        self.scale = dim ** -0.5 if scale is None else scale
         self.data, self.gc = on_gpu(self.cache)
         self.d = {"q": dev(self.q), "start": dev(self.start), "len": dev(self.lens, np.int32), "table": dev(self.table),
                   "prefix": dev(self.prefix_pages) if prefix else None}
         self.out = torch.full((self.tokens, heads, dim), 5.0, device="cuda:0")
-        self.att = G.Attention(self.gc, heads=heads, max_tokens=max(self.tokens, len(lens)), max_q_len=max(self.new), scale=self.scale,
+        self.att = G.Attention(self.gc, heads=heads, max_tokens=max(self.tokens, len(lens)), max_q_len=hint or max(self.new), scale=self.scale,
                                prefix_len=prefix)
         self.ws = torch.full((max(self.att.workspace_bytes, 1),), 255, dtype=torch.uint8, device="cuda:0")
         self.stream = torch.cuda.Stream()
@@ -304,6 +304,37 @@ def test_attention_bounds_lengths(kind):
     c.call()
     c.stream.synchronize()
     c.check(lens=[64, 0, 20])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new,hint", [([70, 3], 1), ([1, 1], 60), ([70, 3], 2)])
+def test_attention_whatever_length_is_announced(kind, new, hint):
+    """More new tokens than max_q_len, or far fewer: the other kernels, the same answer."""
+    AttnCase(31, kind, 8, 2, 128, 16, [200, 130], new, prefix=40, pad=60 if hint > 2 else 0, hint=hint).run()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new,prefix", [([1, 4], 0), ([40, 2], 33), ([1, 1], 200)])
+def test_attention_leaves_rows_of_no_sequence(kind, new, prefix):
+    """q_start may begin behind rows that belong to nobody."""
+    AttnCase(32, kind, 8, 2, 128, 16, [50, 77], new, prefix=prefix, pad=2, before=5).run()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("scale", [0.0, -0.1])
+@pytest.mark.parametrize("new", [[1, 2], [60, 2]])
+def test_attention_scale_of_any_sign(kind, scale, new):
+    AttnCase(33, kind, 8, 2, 128, 16, [90, 300], new, prefix=20, scale=scale).run()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new", [[1, 2], [60, 2]])
+def test_attention_skips_prefix_pages_outside_the_cache(kind, new):
+    c = AttnCase(34, kind, 8, 2, 128, 16, [70, 9], new, prefix=100)
+    c.prefix_pages[[0, 3, 6]] = -1, c.cache.n_pages, 2 ** 31 - 1
+    c.d["prefix"].copy_(dev(c.prefix_pages))
+    torch.cuda.synchronize()
+    c.run()
 
 
 def test_attention_large_scores_and_flat_rows():
@@ -455,6 +486,34 @@ def test_sample_infinite_and_missing_logits():
     for t in (0.0, 1.0, 1e-30, math.inf, math.nan, -1.0):
         check_ids(x, [0.5, 0.99, 0.0, 0.3, 0.7, 0.5, 0.999, 0.5, 0.25], t=[t] * 9, k=[2] * 9, p=[0.9] * 9)
         check_ids(x, [0.5, 0.99, 0.0, 0.3, 0.7, 0.5, 0.999, 0.5, 0.25], t=[t] * 9)
+
+
+def test_sample_without_shares():
+    x = np.random.default_rng(9).normal(size=(3, 500)).astype(np.float32)
+    d, u, ids = dev(x), dev([0.1, 0.5, 0.9], np.float32), torch.zeros(3, dtype=torch.int32, device="cuda:0")
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    G.sample_dev(ids.data_ptr(), d.data_ptr(), 3, 500, u.data_ptr(), stream=st.cuda_stream)
+    st.synchronize()
+    assert ids.tolist() == [sample(x[r], u[r].item(), 1.0, 0, 1.0, 0.0)[0] for r in range(3)]
+
+
+def test_nothing_to_do_is_no_error():
+    cache = Cache(G.TYPE_F16, 2, 16, 1, 64)
+    data, gc = on_gpu(cache)
+    t = torch.zeros(64, device="cuda:0")
+    p = t.data_ptr()
+    G.kv_write_dev(gc, p, p, p, 0)
+    G.kv_read_dev(gc, p, p, p, 0)
+    G.sample_dev(p, p, 0, 10, p)
+    a = G.Attention(gc, heads=1, max_tokens=4, scale=1.0)
+    ws = torch.zeros(a.workspace_bytes, dtype=torch.uint8, device="cuda:0")
+    a(p, p, 0, 0, p, p, 1, ws.data_ptr(), ws.numel(), q_start_ptr=p)
+    with pytest.raises(G.GoInferCudaError) as e:
+        a(p, p, 1, 1, p, p, 1, ws.data_ptr(), ws.numel() - 1)
+    assert e.value.code == G.ERR_SHAPE and "workspace" in str(e.value)
+    torch.cuda.synchronize()
+    assert not data.any() and not t.any()
 
 
 def test_sample_borders_of_u_and_parameters():
