@@ -17,6 +17,11 @@ GI_DEVINL float exp2_approx(float x) {
   return r;
 }
 
+// 16 bytes to shared memory, of which the first `bytes` (16 or 0) are read.
+GI_DEVINL void cp_async16_or_zero(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
 // Four int8 codes as two half2 (exact): 0x6400 + (c + 128) is the half
 // 1152 + c.
 GI_DEVINL void codes_to_h2(uint32_t w, uint32_t& lo, uint32_t& hi) {

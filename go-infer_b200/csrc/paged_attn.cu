@@ -51,11 +51,6 @@ constexpr int kMergeThreads = 128;
 // took 135 us instead of 127.
 constexpr int kUnitCost = 8;
 
-// 16 bytes to shared memory, of which the first `bytes` (16 or 0) are read.
-GI_DEVINL void cp_async16_or_zero(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
 GI_DEVINL void ldsm_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)

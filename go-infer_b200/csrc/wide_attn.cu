@@ -13,14 +13,17 @@
 //   warps 0-7    softmax: row 32 (w % 4) + lane, positions 64 (w / 4) + 0..63
 //                of the tile; also the queries, the running sums, the output
 //   warps 8-11   K, 12-14 V^T: the tiles' groups of 16 positions in turn, global
-//                -> registers (a group ahead) -> shared memory, 128-byte swizzle
+//                -> a ring of raw groups (cp.async) -> halves in the operand
+//                tiles, 128-byte swizzle
 //   warp 15      tcgen05.mma (one thread), tensor memory
 // (16 warps: a thread can have 128 registers)
-// K and V^T are K-major operands: V is transposed on its way through the
+// K and V^T are K-major operands: V is transposed on its way through
 // registers, where Q8_0 codes become halves in any case.  P takes the place
 // of S in tensor memory (16 columns of S become 8 of high and 8 of low
 // halves) and is the A operand of P V from there.
-// Tensor memory: S/P twice, P V twice, 128 columns each at most.
+// Tensor memory, 128 columns each: S/P twice, P V, the queries' high and low
+// halves (the A operand of S, so that an S product reads only K from shared
+// memory).
 // P V of one tile starts from zero; the running sum over tiles is a float32
 // FMA in the softmax threads' registers, so rounding does not grow with the
 // length (the tensor cores cut their sums).
@@ -45,12 +48,16 @@ constexpr int kWideThreads = 32 * (kSoftWarps + kLoadWarps + 1);
 constexpr int kWideCost = 2;  // tiles that a unit's start and end take
 constexpr int kTmem = 512;
 
-template <int HD>
+template <int HD, int TYPE>
 struct Wide {
-  static constexpr int kOperand = kRows * HD * 2;      // bytes of Q's high (or low) part, of K
-  static constexpr int kV = HD * kTok * 2;             // bytes of V^T: two sub-tiles of 64 positions
-  static constexpr int kQ = 0, kK = 2 * kOperand, kVt = kK + 2 * kOperand;
-  static constexpr int kEnd = kVt + 2 * kV;
+  static constexpr int kElem = TYPE == kTypeF16 ? 2 : 1;
+  static constexpr int kOperand = kTok * HD * 2;       // bytes of a K tile: sub-tiles of 64 dimensions
+  static constexpr int kV = HD * kTok * 2;             // bytes of a V^T tile: two sub-tiles of 64 positions
+  static constexpr int kData = 16 * HD * kElem;        // bytes of a group of 16 positions in the cache
+  static constexpr int kSlot = kData + (TYPE == kTypeF16 ? 0 : HD);  // with its scales
+  static constexpr int kSlots = TYPE == kTypeF16 ? 2 : 4;            // groups a loading warp has in flight
+  static constexpr int kK = 0, kVt = 2 * kOperand, kRing = kVt + 2 * kV;
+  static constexpr int kEnd = kRing + kLoadWarps * kSlots * kSlot;
   static constexpr int kSmem = kEnd + 1024 /* alignment */ + 8192;
   static constexpr int kPart = kRows * (HD + 2);
   static constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kTok >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
@@ -88,13 +95,6 @@ GI_DEVINL void tmem_ld32(uint32_t taddr, float (&v)[32]) {
 // the warp computes the operands' descriptors together, in uniform
 // registers, and only the instruction itself is predicated.  Issued from
 // inside an `if (lane == 0)` each product costs some 130 clocks of moves.
-GI_DEVINL void mma_by(uint32_t mine, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{ .reg .pred p, q; setp.ne.b32 p, %4, 0; setp.ne.b32 q, %5, 0; "
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(mine)
-      : "memory");
-}
 GI_DEVINL void mma_ts_by(uint32_t mine, uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{ .reg .pred p, q; setp.ne.b32 p, %4, 0; setp.ne.b32 q, %5, 0; "
@@ -172,21 +172,20 @@ __device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int
 // quarter of the speed.
 template <int HD, int TYPE>
 __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p, int* error) {
-  using W = Wide<HD>;
+  using W = Wide<HD, TYPE>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023) & ~1023u;
   uint8_t* sm = smem_raw + (base - raw);
   float2* s_ml = reinterpret_cast<float2*>(sm + W::kEnd);          // [2][row]: a half row's statistics
   float* s_max = reinterpret_cast<float*>(s_ml + 2 * kRows);       // [tile parity][half][row]
-  float* s_fac = s_max + 4 * kRows;                                // [row]
-  uint8_t* s_bad = reinterpret_cast<uint8_t*>(s_fac + kRows);      // [tile % 4][16-position group]
+  uint8_t* s_bad = reinterpret_cast<uint8_t*>(s_max + 4 * kRows);  // [tile % 4][16-position group]
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_bad + 32);
   volatile int* s_stop = reinterpret_cast<volatile int*>(s_tmem + 1);
   const uint32_t bars = smem_u32(s_tmem + 4);  // 8-byte aligned: everything above is a multiple of 16 bytes
   Unit* s_unit = reinterpret_cast<Unit*>(s_tmem + 4 + 2 * 18);  // the softmax warps' unit
   // barriers, [tile parity] each but the queries'
   auto k_full = [&](int i) { return bars + 8 * i; };
-  auto pv_full = [&](int i) { return bars + 8 * (2 + i); };  // V^T is there and P: P comes after the row's P V of two tiles before is taken
+  auto pv_full = [&](int i) { return bars + 8 * (2 + i); };  // V^T is there and P, which comes after P V of the tile before is taken
   auto k_free = [&](int i) { return bars + 8 * (4 + i); };
   auto v_free = [&](int i) { return bars + 8 * (6 + i); };
   auto s_full = [&](int i) { return bars + 8 * (8 + i); };
@@ -224,7 +223,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(s_tmem);
   auto s_col = [&](int i) { return tmem + i * kTok; };
-  auto o_col = [&](int i) { return tmem + 2 * kTok + i * 128; };
+  const uint32_t o_col = tmem + 2 * kTok, q_col = o_col + 128;  // P V; the queries' high, then low halves
 
   // By every lane of a warp, which leaves together; false ends the role.
   auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -254,13 +253,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
           tc_fence_after();
           const int buf = __shfl_sync(0xffffffffu, n & 1, 0);
           const uint32_t d = tmem_u + buf * kTok;
-          const uint64_t q = desc_sw128(base + W::kQ), k = desc_sw128(base + W::kK + buf * W::kOperand);
+          const uint32_t q = tmem_u + 2 * kTok + 128;
+          const uint64_t k = desc_sw128(base + W::kK + buf * W::kOperand);
 #pragma unroll
           for (int part = 0; part < 2; ++part)  // the low halves first: each step cuts the sum, and theirs is small
 #pragma unroll
             for (int e = 0; e < HD / 16; ++e) {
-              const int off = (e >> 2) * (kRows * 128 / 16) + (e & 3) * 2;
-              mma_by(mine, d, q + (1 - part) * (W::kOperand / 16) + off, k + off, W::kIdescS, part | e);
+              const int off = (e >> 2) * (kTok * 128 / 16) + (e & 3) * 2;
+              mma_ts_by(mine, d, q + (1 - part) * (HD / 2) + 8 * e, k + off, W::kIdescS, part | e);
             }
           commit_by(mine, s_full(buf));
           commit_by(mine, k_free(buf));
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
           if (!ok) break;
           tc_fence_after();
           const int buf = __shfl_sync(0xffffffffu, n & 1, 0);
-          const uint32_t d = tmem_u + 2 * kTok + buf * 128, a = tmem_u + buf * kTok;
+          const uint32_t d = tmem_u + 2 * kTok, a = tmem_u + buf * kTok;
           const uint64_t v = desc_sw128(base + W::kVt + buf * W::kV);
 #pragma unroll
           for (int part = 0; part < 2; ++part)
@@ -292,198 +292,161 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
     }
     __syncwarp();
   } else if (warp >= kSoftWarps) {
-    // ---- operand tiles: a warp takes every 4th group of K, or every 3rd of V, the next group's loads in flight ----
-    constexpr int kE = TYPE == kTypeF16 ? 2 : 1;
-    constexpr int kKLoads = 16 * HD * kE / 512;  // 16-byte loads of K per lane
+    // ---- operand tiles: a warp takes every 4th group of K, or every 3rd of V ----
+    constexpr int kE = W::kElem;
+    constexpr int kLoads = W::kData / 512;       // 16-byte copies of a group per lane
     constexpr int kDims = HD / 32;               // dimensions of V per lane
     constexpr int kVWords = kDims * kE >= 4 ? kDims * kE / 4 : 1;
     constexpr int kScaleWords = HD / 64;  // words of a position's scales
     const bool is_k = warp < kSoftWarps + kKWarps;
     const int step = is_k ? kKWarps : kVWarps, id = is_k ? warp - kSoftWarps : warp - kSoftWarps - kKWarps;
+    const uint32_t slots = base + W::kRing + (warp - kSoftWarps) * W::kSlots * W::kSlot;
     // The warp's groups of a unit in turn: group g of the unit's 8 * tiles is
-    // its if (8 tile_no + g) % step == id.  32 pages are looked up at a time,
-    // one per lane, so that a group's loads do not wait for its page.
-    struct Group {
-      const uint8_t* src;
-      int left;         // positions of the 16 that exist
-      bool bad;         // no such page
-      uint32_t scales;  // Q8_0: word `lane` of the 16 positions' scales
-    };
+    // its if (8 tile_no + g) % step == id.  kSlots of them are on their way
+    // into the warp's slots; 32 pages are looked up at a time, one per lane, so
+    // that a group's copies do not wait for its page.
     int page = 0, page_of = 0;  // of group page_of + lane * step
+    uint32_t bads = 0;          // bit s: slot s's group has no such page
     auto look_up = [&](int g) {
       page_of = g;
       const int p0 = u.tile0 * kTok + 16 * (g + lane * step);
       const int32_t* pages = p.pages + (p.prefix ? 0 : (size_t)u.b * p.pages_stride);
       page = p0 < u.s.len && p0 >= 0 ? __ldg(pages + (p0 >> c.page_shift)) : 0;
     };
-    auto group_at = [&](int g) {
-      Group x;
+    auto copy = [&](int g, int slot) {
       if (g >= page_of + 32 * step) look_up(g);
       const int p0 = u.tile0 * kTok + 16 * g, pg = __shfl_sync(0xffffffffu, page, (g - page_of) / step);
-      x.bad = (unsigned)pg >= (unsigned)c.n_pages;
-      x.left = x.bad ? 0 : u.s.len - p0;
-      const size_t at = (((size_t)(x.bad ? 0 : pg) * c.n_kv_heads + u.h) << c.page_shift) + (p0 & (c.page_size - 1));
-      x.src = (is_k ? c.k : c.v) + at * HD * kE;
-      x.scales = 0u;
-      if (TYPE == kTypeQ8_0 && lane < 16 * kScaleWords && lane / kScaleWords < x.left)
-        x.scales = __ldg(reinterpret_cast<const uint32_t*>((is_k ? c.ks : c.vs) + at * (HD / 32)) + lane);
-      return x;
+      const bool bad = (unsigned)pg >= (unsigned)c.n_pages;
+      bads = (bads & ~(1u << slot)) | (uint32_t)bad << slot;
+      const int left = bad ? 0 : u.s.len - p0;
+      const size_t at = (((size_t)(bad ? 0 : pg) * c.n_kv_heads + u.h) << c.page_shift) + (p0 & (c.page_size - 1));
+      const uint8_t* src = (is_k ? c.k : c.v) + at * HD * kE;
+      const uint32_t dst = slots + slot * W::kSlot;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int ch = 32 * i + lane;
+        cp_async16_or_zero(dst + 16 * ch, src + 16 * ch, ch / (HD * kE / 16) < left ? 16 : 0);
+      }
+      if (TYPE == kTypeQ8_0 && lane < HD / 16)  // 16 bytes: the scales of 256 / HD positions
+        cp_async16_or_zero(dst + W::kData + 16 * lane,
+                           reinterpret_cast<const uint8_t*>(is_k ? c.ks : c.vs) + at * (HD / 16) + 16 * lane,
+                           16 * lane < left * (HD / 16) ? 16 : 0);
+    };
+    // word `lane` of a slot's scales; 0 for positions that do not exist, whatever lies there
+    auto scales_of = [&](int g, int slot) {
+      uint32_t w = 0;
+      if (TYPE == kTypeQ8_0 && lane < 16 * kScaleWords &&
+          u.tile0 * kTok + 16 * g + lane / kScaleWords < ((bads >> slot) & 1 ? 0 : u.s.len))
+        w = lds32(slots + slot * W::kSlot + W::kData + 4 * lane);
+      return w;
     };
     // scale of position r, block b, from the lanes' words
     auto scale_word = [&](uint32_t words, int r, int b) {
       return __shfl_sync(0xffffffffu, words, r * kScaleWords + (b >> 1));
     };
-    if (is_k) {
-      uint4 kr[kKLoads], kn[kKLoads];  // the group at hand, the next
-      Group gr, gn;
-      auto load = [&](uint4 (&x)[kKLoads], const Group& y) {
+    auto put_k = [&](uint32_t from, uint32_t scales, int tile, int w) {
+      const uint32_t dst = base + W::kK + (tile & 1) * W::kOperand;
 #pragma unroll
-        for (int i = 0; i < kKLoads; ++i) {
-          const int ch = 32 * i + lane;
-          x[i] = ch / (HD * kE / 16) < y.left ? ldg_stream(y.src + 16 * ch) : make_uint4(0, 0, 0, 0);
-        }
-      };
-      auto put = [&](const uint4 (&x)[kKLoads], const Group& y, int tile, int w) {
-        const uint32_t dst = base + W::kK + (tile & 1) * W::kOperand;
+      for (int l = 0; l < kLoads; ++l) {
+        const int ch = 32 * l + lane, per = HD * kE / 16, r = ch / per, row = 16 * w + r, q = ch - r * per;
+        const uint4 x = lds128(from + 16 * ch);
+        if (TYPE == kTypeF16) {  // 8 values: one 16-byte unit
+          sts128(dst + (q >> 3) * (kTok * 128) + sw128_off(row, q & 7), x.x, x.y, x.z, x.w);
+        } else {  // 16 codes: two units, all of one block
+          const int b = q >> 1;
+          const uint32_t d2 = prmt(scale_word(scales, r, b), 0u, b & 1 ? 0x3232 : 0x1010);
+          uint32_t o[8];
+          codes_to_h2(x.x, o[0], o[1]);
+          codes_to_h2(x.y, o[2], o[3]);
+          codes_to_h2(x.z, o[4], o[5]);
+          codes_to_h2(x.w, o[6], o[7]);
 #pragma unroll
-        for (int l = 0; l < kKLoads; ++l) {
-          const int ch = 32 * l + lane, per = HD * kE / 16, r = ch / per, row = 16 * w + r, q = ch - r * per;
-          if (TYPE == kTypeF16) {  // 8 values: one 16-byte unit
-            sts128(dst + (q >> 3) * (kTok * 128) + sw128_off(row, q & 7), x[l].x, x[l].y, x[l].z, x[l].w);
-          } else {  // 16 codes: two units, all of one block
-            const int b = q >> 1;
-            const uint32_t d2 = prmt(scale_word(y.scales, r, b), 0u, b & 1 ? 0x3232 : 0x1010);
-            uint32_t o[8];
-            codes_to_h2(x[l].x, o[0], o[1]);
-            codes_to_h2(x[l].y, o[2], o[3]);
-            codes_to_h2(x[l].z, o[4], o[5]);
-            codes_to_h2(x[l].w, o[6], o[7]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = hmul2_u32(o[e], d2);
-            const uint32_t t = dst + (q >> 2) * (kTok * 128);
-            const int unit = 2 * (q & 3);
-            sts128(t + sw128_off(row, unit), o[0], o[1], o[2], o[3]);
-            sts128(t + sw128_off(row, unit + 1), o[4], o[5], o[6], o[7]);
-          }
+          for (int e = 0; e < 8; ++e) o[e] = hmul2_u32(o[e], d2);
+          const uint32_t t = dst + (q >> 2) * (kTok * 128);
+          const int unit = 2 * (q & 3);
+          sts128(t + sw128_off(row, unit), o[0], o[1], o[2], o[3]);
+          sts128(t + sw128_off(row, unit + 1), o[4], o[5], o[6], o[7]);
         }
-      };
-      bool go = true;
-      while (go && walk.next(c, p, group, &u)) {
-        const int n_groups = u.tiles * kGroups;
-        const int g0 = ((id - tile_no * kGroups) % step + step) % step;  // this warp's first
-        if (g0 < n_groups) look_up(g0);
-        if (g0 < n_groups) {
-          gr = group_at(g0);
-          load(kr, gr);
-        }
-        if (g0 + step < n_groups) {
-          gn = group_at(g0 + step);
-          load(kn, gn);
-        }
-#pragma unroll 1
-        for (int g = g0; g < n_groups; g += step) {
-          const int n = tile_no + g / kGroups, w = g % kGroups;
-          if (!(go = wait(k_free(n & 1), phase(n) ^ 1))) break;
-          if (lane == 0) s_bad[8 * (n & 3) + w] = gr.bad;  // read until the softmax of this tile is done
-          put(kr, gr, n, w);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(k_full(n & 1));
-          gr = gn;
-#pragma unroll
-          for (int i = 0; i < kKLoads; ++i) kr[i] = kn[i];
-          if (g + 2 * step < n_groups) {
-            gn = group_at(g + 2 * step);
-            load(kn, gn);
-          }
-        }
-        tile_no += u.tiles;
       }
-    } else {
-      uint32_t vr[16][kVWords], vn[16][kVWords];
-      Group gr, gn;
-      auto load = [&](uint32_t (&x)[16][kVWords], const Group& y) {
+    };
+    auto put_v = [&](uint32_t from, uint32_t scales, int tile, int w) {
+      // 64 positions per sub-tile
+      const uint32_t dst = base + W::kVt + (tile & 1) * W::kV + (w >> 2) * (HD * 128);
+      const int b = lane * kDims / 32;  // this lane's block of 32 dimensions
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const uint8_t* a = y.src + (size_t)r * HD * kE + lane * kDims * kE;
+      for (int half = 0; half < 2; ++half) {  // 8 positions: one 16-byte unit of each of the lane's rows
+        uint32_t x[8][kVWords], o[kDims][4];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const uint32_t a = from + (8 * half + r) * HD * kE + lane * kDims * kE;
           if (kDims * kE == 8) {
-            const uint2 z = r < y.left ? __ldg(reinterpret_cast<const uint2*>(a)) : make_uint2(0, 0);
-            x[r][0] = z.x;
-            x[r][kVWords - 1] = z.y;
-          } else if (kDims * kE == 4) {
-            x[r][0] = r < y.left ? ldg_stream32(a) : 0u;
-          } else {  // two codes
-            x[r][0] = r < y.left ? (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(a)) : 0u;
+            const uint64_t z = lds64(a);
+            x[r][0] = (uint32_t)z;
+            x[r][kVWords - 1] = (uint32_t)(z >> 32);
+          } else {
+            x[r][0] = kDims * kE == 4 ? lds32(a) : lds16(a);
           }
         }
-      };
-      auto put = [&](const uint32_t (&x)[16][kVWords], const Group& y, int tile, int w) {
-        // 64 positions per sub-tile
-        const uint32_t dst = base + W::kVt + (tile & 1) * W::kV + (w >> 2) * (HD * 128);
-        const int b = lane * kDims / 32;  // this lane's block of 32 dimensions
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {  // 8 positions: one 16-byte unit of each of the lane's rows
-          uint32_t o[kDims][4];
+        for (int q = 0; q < 4; ++q) {
+          if (TYPE == kTypeF16) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+            for (int e = 0; e < kDims / 2; ++e) {
+              o[2 * e][q] = prmt(x[2 * q][e], x[2 * q + 1][e], 0x5410);
+              o[2 * e + 1][q] = prmt(x[2 * q][e], x[2 * q + 1][e], 0x7632);
+            }
+          } else {
             const int r = 8 * half + 2 * q;
-            if (TYPE == kTypeF16) {
-#pragma unroll
-              for (int e = 0; e < kDims / 2; ++e) {
-                o[2 * e][q] = prmt(x[r][e], x[r + 1][e], 0x5410);
-                o[2 * e + 1][q] = prmt(x[r][e], x[r + 1][e], 0x7632);
-              }
-            } else {
-              const uint32_t d = prmt(scale_word(y.scales, r, b), scale_word(y.scales, r + 1, b), b & 1 ? 0x7632 : 0x5410);
-              uint32_t x0, x1;
-              codes_to_h2(prmt(x[r][0], x[r + 1][0], 0x5140), x0, x1);
-              o[0][q] = hmul2_u32(x0, d);
-              o[1][q] = hmul2_u32(x1, d);
-              if (kDims == 4) {
-                codes_to_h2(prmt(x[r][0], x[r + 1][0], 0x7362), x0, x1);
-                o[2 % kDims][q] = hmul2_u32(x0, d);
-                o[3 % kDims][q] = hmul2_u32(x1, d);
-              }
+            const uint32_t d = prmt(scale_word(scales, r, b), scale_word(scales, r + 1, b), b & 1 ? 0x7632 : 0x5410);
+            uint32_t x0, x1;
+            codes_to_h2(prmt(x[2 * q][0], x[2 * q + 1][0], 0x5140), x0, x1);
+            o[0][q] = hmul2_u32(x0, d);
+            o[1][q] = hmul2_u32(x1, d);
+            if (kDims == 4) {
+              codes_to_h2(prmt(x[2 * q][0], x[2 * q + 1][0], 0x7362), x0, x1);
+              o[2 % kDims][q] = hmul2_u32(x0, d);
+              o[3 % kDims][q] = hmul2_u32(x1, d);
             }
           }
+        }
 #pragma unroll
-          for (int e = 0; e < kDims; ++e)
-            sts128(dst + sw128_off(lane * kDims + e, 2 * (w & 3) + half), o[e][0], o[e][1], o[e][2], o[e][3]);
-        }
-      };
-      bool go = true;
-      while (go && walk.next(c, p, group, &u)) {
-        const int n_groups = u.tiles * kGroups;
-        const int g0 = ((id - tile_no * kGroups) % step + step) % step;  // this warp's first
-        if (g0 < n_groups) look_up(g0);
-        if (g0 < n_groups) {
-          gr = group_at(g0);
-          load(vr, gr);
-        }
-        if (g0 + step < n_groups) {
-          gn = group_at(g0 + step);
-          load(vn, gn);
-        }
-#pragma unroll 1
-        for (int g = g0; g < n_groups; g += step) {
-          const int n = tile_no + g / kGroups, w = g % kGroups;
-          if (!(go = wait(v_free(n & 1), phase(n) ^ 1))) break;
-          put(vr, gr, n, w);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(pv_full(n & 1));
-          gr = gn;
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-#pragma unroll
-            for (int i = 0; i < kVWords; ++i) vr[r][i] = vn[r][i];
-          if (g + 2 * step < n_groups) {
-            gn = group_at(g + 2 * step);
-            load(vn, gn);
-          }
-        }
-        tile_no += u.tiles;
+        for (int e = 0; e < kDims; ++e)
+          sts128(dst + sw128_off(lane * kDims + e, 2 * (w & 3) + half), o[e][0], o[e][1], o[e][2], o[e][3]);
       }
+    };
+    bool go = true;
+    while (go && walk.next(c, p, group, &u)) {
+      const int n_groups = u.tiles * kGroups;
+      const int g0 = ((id - tile_no * kGroups) % step + step) % step;  // this warp's first
+      if (g0 < n_groups) look_up(g0);
+#pragma unroll 1
+      for (int s = 0; s < W::kSlots; ++s) {
+        if (g0 + s * step < n_groups) copy(g0 + s * step, s);
+        cp_async_commit();
+      }
+      int slot = 0;
+#pragma unroll 1
+      for (int g = g0; g < n_groups; g += step) {
+        const int n = tile_no + g / kGroups, w = g % kGroups;
+        cp_async_wait<W::kSlots - 1>();
+        __syncwarp();
+        if (!(go = wait(is_k ? k_free(n & 1) : v_free(n & 1), phase(n) ^ 1))) break;
+        const uint32_t from = slots + slot * W::kSlot, scales = scales_of(g, slot);
+        if (is_k) {
+          if (lane == 0) s_bad[8 * (n & 3) + w] = (bads >> slot) & 1;  // read until the softmax of this tile is done
+          put_k(from, scales, n, w);
+        } else {
+          put_v(from, scales, n, w);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(is_k ? k_full(n & 1) : pv_full(n & 1));
+        if (g + W::kSlots * step < n_groups) copy(g + W::kSlots * step, slot);
+        cp_async_commit();
+        slot = slot + 1 == W::kSlots ? 0 : slot + 1;
+      }
+      cp_async_wait<0>();
+      tile_no += u.tiles;
     }
   } else {
     // ---- softmax ----
@@ -501,136 +464,139 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
       const int tiles = s_unit->tiles;
       if (tiles < 0) break;
       // queries: a power of two per row that puts the largest just under 2^14, then
-      // high and low halves.  HD / 4 lanes read a row, four dimensions each.
+      // high and low halves into tensor memory, the A operand of S
+      float fac;
       {
-        const int row0 = s_unit->row0, n_rows = s_unit->n_rows;
-        const float* q0 = p.q + ((size_t)s_unit->s.start * p.n_heads + (size_t)s_unit->h * group) * HD;
-        constexpr int kPer = HD / 4, kAtOnce = 128 / HD, kBatch = 8;  // lanes per row; rows per load; loads in flight
-        const int d = 4 * (lane % kPer);
-        // the warp's 16 rows, one per lane: their places in q
-        const int my = row0 + warp * 16 + (lane & 15);
-        const int place = (my / group) * p.n_heads + my % group;  // n_tokens * n_heads fits an int
-        for (int r0 = warp * 16; r0 < warp * 16 + 16; r0 += kBatch * kAtOnce) {
-          float4 x[kBatch];
+        const int row = s_unit->row0 + r;
+        const bool real = r < s_unit->n_rows;
+        const float4* q = reinterpret_cast<const float4*>(
+            p.q + ((size_t)(s_unit->s.start + (real ? row / group : 0)) * p.n_heads + (size_t)s_unit->h * group +
+                   (real ? row % group : 0)) * HD + half * kOut);
+        float x[kOut], m = 0.f;
 #pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            const int qr = r0 + i * kAtOnce + lane / kPer;
-            const float* q = q0 + (size_t)__shfl_sync(0xffffffffu, place, qr & 15) * HD;
-            x[i] = qr < n_rows ? __ldg(reinterpret_cast<const float4*>(q + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
-          }
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            const int qr = r0 + i * kAtOnce + lane / kPer;
-            float m = fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w)));
-#pragma unroll
-            for (int o = kPer / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const int ex = (int)(__float_as_uint(m) >> 23) - 127;
-            const int sh = m > 0.f ? min(13 - ex, 126) : 0;
-            const float up = p.scale < 0.f ? -exp2i(sh) : exp2i(sh);  // the scale's sign with q: the factor on S is >= 0
-            if (lane % kPer == 0) s_fac[qr] = fabsf(p.scale) * kLog2e * exp2i(-sh);
-            const float y[4] = {x[i].x * up, x[i].y * up, x[i].z * up, x[i].w * up};
-            uint32_t hi[2], lo[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              hi[e] = pack_h2(y[2 * e], y[2 * e + 1]);
-              const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-              lo[e] = pack_h2(y[2 * e] - back.x, y[2 * e + 1] - back.y);
-            }
-            const uint32_t off = base + W::kQ + (d >> 6) * (kRows * 128) + sw128_off(qr, (d & 63) >> 3) + (d & 4) * 2;
-            sts64(off, (uint64_t)hi[1] << 32 | hi[0]);
-            sts64(off + W::kOperand, (uint64_t)lo[1] << 32 | lo[0]);
-          }
+        for (int i = 0; i < kOut / 4; ++i) {
+          const float4 y = real ? __ldg(q + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+          x[4 * i] = y.x, x[4 * i + 1] = y.y, x[4 * i + 2] = y.z, x[4 * i + 3] = y.w;
         }
-        fence_proxy_async_smem();
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) m = fmaxf(m, fabsf(x[i]));
+        s_max[half * kRows + r] = m;
         soft_sync();
+        m = fmaxf(m, s_max[(half ^ 1) * kRows + r]);
+        const int ex = (int)(__float_as_uint(m) >> 23) - 127;
+        const int sh = m > 0.f ? min(13 - ex, 126) : 0;
+        const float up = p.scale < 0.f ? -exp2i(sh) : exp2i(sh);  // the scale's sign with q: the factor on S is >= 0
+        fac = fabsf(p.scale) * kLog2e * exp2i(-sh);
+#pragma unroll
+        for (int i = 0; i < kOut; i += 32) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float x0 = x[i + 2 * e] * up, x1 = x[i + 2 * e + 1] * up;
+            hi[e] = pack_h2(x0, x1);
+            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+            lo[e] = pack_h2(x0 - back.x, x1 - back.y);
+          }
+          const uint32_t to = q_col + lanes + (half * kOut + i) / 2;
+          tmem_st16(to, hi);
+          tmem_st16(to + HD / 2, lo);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        soft_sync();  // s_max is read
         if (lane == 0) mbar_arrive(q_full);
       }
-      const float fac = s_fac[r];
       const int seen = seen_by(p, s_unit->s, (s_unit->row0 + min(r, s_unit->n_rows - 1)) / group) - s_unit->tile0 * kTok;
       const int seen_first = s_unit->seen_first - s_unit->tile0 * kTok;  // positions from the first tile's on
       float o[kOut], m = -INFINITY, l = 0.f, alpha = 0.f;
 #pragma unroll
       for (int i = 0; i < kOut; ++i) o[i] = 0.f;
       for (int i = 0; i <= tiles && ok && tiles; ++i) {
-        float alpha_n = 0.f;
-        if (i < tiles) {
-        const int n = tile_no + i, p0 = i * kTok + 64 * half;
-        if (!(ok = wait(s_full(n & 1), phase(n)))) break;
-        tc_fence_after();
-        const uint32_t bad = *reinterpret_cast<const volatile uint32_t*>(s_bad + 8 * (n & 3) + 4 * half);
-        const bool masked = p0 + 64 > seen_first || bad;  // uniform in the warp
-        const uint32_t s = s_col(n & 1) + lanes + 64 * half;
+        const int n_i = tile_no + i, p0 = i * kTok + 64 * half;
+        const uint32_t s = s_col(n_i & 1) + lanes + 64 * half;
+        uint32_t bad = 0;
+        bool masked = false;
+        float alpha_n = 0.f, zero = 0.f;
         // positions j .. j + 15 of the 64 that this row sees
         auto limit = [&](int j) { return (bad >> (8 * (j >> 4))) & 1 ? 0 : seen - p0 - j; };
-        float top = -INFINITY;
+        if (i < tiles) {
+          const int n = n_i;
+          if (!(ok = wait(s_full(n & 1), phase(n)))) break;
+          tc_fence_after();
+          bad = *reinterpret_cast<const volatile uint32_t*>(s_bad + 8 * (n & 3) + 4 * half);
+          masked = p0 + 64 > seen_first || bad;  // uniform in the warp
+          float top = -INFINITY;
 #pragma unroll 1
-        for (int j = 0; j < 64; j += 32) {
-          float x[32];
-          tmem_ld32(s + j, x);
-          if (masked) {
-            const int l0 = limit(j), l1 = limit(j + 16);
+          for (int j = 0; j < 64; j += 32) {
+            float x[32];
+            tmem_ld32(s + j, x);
+            if (masked) {
+              const int l0 = limit(j), l1 = limit(j + 16);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              x[e] = e < l0 ? x[e] : -INFINITY;
-              x[16 + e] = e < l1 ? x[16 + e] : -INFINITY;
+              for (int e = 0; e < 16; ++e) {
+                x[e] = e < l0 ? x[e] : -INFINITY;
+                x[16 + e] = e < l1 ? x[16 + e] : -INFINITY;
+              }
             }
-          }
-          float t2 = x[1];
+            float t2 = x[1];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            top = fmaxf(top, x[e]);
-            t2 = fmaxf(t2, x[e + 1]);
+            for (int e = 0; e < 32; e += 2) {
+              top = fmaxf(top, x[e]);
+              t2 = fmaxf(t2, x[e + 1]);
+            }
+            top = fmaxf(top, t2);
           }
-          top = fmaxf(top, t2);
+          s_max[((n & 1) * 2 + half) * kRows + r] = top;
+          soft_sync();
+          top = fmaxf(top, s_max[((n & 1) * 2 + (half ^ 1)) * kRows + r]);
+          const float mn = top == -INFINITY ? m : fmaxf(m, top * fac);
+          zero = mn == -INFINITY ? 0.f : mn;
+          alpha_n = exp2_approx(m - zero);
+          m = mn;
         }
-        s_max[((n & 1) * 2 + half) * kRows + r] = top;
-        soft_sync();
-        top = fmaxf(top, s_max[((n & 1) * 2 + (half ^ 1)) * kRows + r]);
-        const float mn = top == -INFINITY ? m : fmaxf(m, top * fac), zero = mn == -INFINITY ? 0.f : mn;
-        alpha_n = exp2_approx(m - zero);
-        m = mn;
-        float sum = 0.f, sum2 = 0.f;
-#pragma unroll 1
-        for (int j = 0; j < 64; j += 16) {
-          float x[16];
-          uint32_t w[16];
-          tmem_ld16(s + j, x);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = exp2_approx(fmaf(x[e], fac, -zero)) * 16384.f;  // not 2^14 in the exponent: 24 bits there lose 2^-21
-          if (masked) {
-            const int l0 = limit(j);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = e < l0 ? x[e] : 0.f;
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            sum += x[2 * e];
-            sum2 += x[2 * e + 1];
-            w[e] = pack_h2(x[2 * e], x[2 * e + 1]);
-            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-            w[8 + e] = pack_h2(x[2 * e] - back.x, x[2 * e + 1] - back.y);
-          }
-          tmem_st16(s + j, w);
-        }
-        sum += sum2;
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(pv_full(n & 1));
-        l = l * alpha_n + sum;
-        }
-        if (i > 0) {  // o = o alpha + P V of the tile before
+        if (i > 0) {  // o = o alpha + P V of the tile before, before this tile's P lets the next one begin
           const int n = tile_no + i - 1;
           if (!(ok = wait(o_full(n & 1), phase(n)))) break;
           tc_fence_after();
 #pragma unroll
           for (int d = 0; d < kOut; d += 32) {
             float x[32];
-            tmem_ld32(o_col(n & 1) + lanes + half * kOut + d, x);
+            tmem_ld32(o_col + lanes + half * kOut + d, x);
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[d + e] = fmaf(o[d + e], alpha, x[e]);
           }
           tc_fence_before();
+        }
+        if (i < tiles) {
+          float sum = 0.f, sum2 = 0.f;
+#pragma unroll 1
+          for (int j = 0; j < 64; j += 16) {
+            float x[16];
+            uint32_t w[16];
+            tmem_ld16(s + j, x);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = exp2_approx(fmaf(x[e], fac, -zero)) * 16384.f;
+            if (masked) {
+              const int l0 = limit(j);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) x[e] = e < l0 ? x[e] : 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              sum += x[2 * e];
+              sum2 += x[2 * e + 1];
+              w[e] = pack_h2(x[2 * e], x[2 * e + 1]);
+              const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+              w[8 + e] = pack_h2(x[2 * e] - back.x, x[2 * e + 1] - back.y);
+            }
+            tmem_st16(s + j, w);
+          }
+          sum += sum2;
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(pv_full(n_i & 1));
+          l = l * alpha_n + sum;
         }
         alpha = alpha_n;
       }
@@ -661,7 +627,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         for (int i = 0; i < kOut; i += 4)
           *reinterpret_cast<float4*>(out + i) = make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
       }
-      soft_sync();  // s_unit, s_ml, s_max and s_fac are read
+      soft_sync();  // s_unit, s_ml and s_max are read
     }
   }
   tc_fence_before();
@@ -673,13 +639,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
 
 template <int HD, int TYPE>
 cudaError_t launch_wide(const KvCache& c, const Pass& p, int sm_count, int* error, cudaStream_t s) {
-  wide_kernel<HD, TYPE><<<sm_count, kWideThreads, Wide<HD>::kSmem, s>>>(c, p, error);
+  wide_kernel<HD, TYPE><<<sm_count, kWideThreads, Wide<HD, TYPE>::kSmem, s>>>(c, p, error);
   return cudaGetLastError();
 }
 
 template <int HD, int TYPE>
 bool prepare_wide() {
-  return cudaFuncSetAttribute(wide_kernel<HD, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Wide<HD>::kSmem) ==
+  return cudaFuncSetAttribute(wide_kernel<HD, TYPE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Wide<HD, TYPE>::kSmem) ==
          cudaSuccess;
 }
 
