@@ -373,37 +373,40 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
       // 64 positions per sub-tile
       const uint32_t dst = base + W::kVt + (tile & 1) * W::kV + (w >> 2) * (HD * 128);
       const int b = lane * kDims / 32;  // this lane's block of 32 dimensions
+      // a lane's rows come in an order of its own, so that eight lanes that store together hold
+      // eight rows that differ mod 8 and with them, by the swizzle, eight 16-byte units of the banks
+      const uint32_t turn = TYPE != kTypeF16 && kDims == 4 ? (lane >> 1) & 3 : (lane >> 2) & 1;
+      const uint32_t first = TYPE == kTypeF16 ? 0x5410 ^ (turn * 0x2222) : (0x5140 ^ (turn * 0x1111));
+      const uint32_t second = first ^ 0x2222;
+      auto row_of = [&](int e) {
+        return TYPE == kTypeF16 ? 64 * (e >> 1) + 2 * lane + ((e & 1) ^ turn) : lane * kDims + (e ^ turn);
+      };
 #pragma unroll
       for (int half = 0; half < 2; ++half) {  // 8 positions: one 16-byte unit of each of the lane's rows
         uint32_t x[8][kVWords], o[kDims][4];
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          const uint32_t a = from + (8 * half + r) * HD * kE + lane * kDims * kE;
-          if (kDims * kE == 8) {
-            const uint64_t z = lds64(a);
-            x[r][0] = (uint32_t)z;
-            x[r][kVWords - 1] = (uint32_t)(z >> 32);
-          } else {
-            x[r][0] = kDims * kE == 4 ? lds32(a) : lds16(a);
-          }
+          const uint32_t a = from + (8 * half + r) * HD * kE + lane * (TYPE == kTypeF16 ? 4 : kDims);
+#pragma unroll
+          for (int i = 0; i < kVWords; ++i) x[r][i] = TYPE != kTypeF16 && kDims == 2 ? lds16(a) : lds32(a + 128 * i);
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           if (TYPE == kTypeF16) {
 #pragma unroll
             for (int e = 0; e < kDims / 2; ++e) {
-              o[2 * e][q] = prmt(x[2 * q][e], x[2 * q + 1][e], 0x5410);
-              o[2 * e + 1][q] = prmt(x[2 * q][e], x[2 * q + 1][e], 0x7632);
+              o[2 * e][q] = prmt(x[2 * q][e], x[2 * q + 1][e], first);
+              o[2 * e + 1][q] = prmt(x[2 * q][e], x[2 * q + 1][e], second);
             }
           } else {
             const int r = 8 * half + 2 * q;
             const uint32_t d = prmt(scale_word(scales, r, b), scale_word(scales, r + 1, b), b & 1 ? 0x7632 : 0x5410);
             uint32_t x0, x1;
-            codes_to_h2(prmt(x[2 * q][0], x[2 * q + 1][0], 0x5140), x0, x1);
+            codes_to_h2(prmt(x[2 * q][0], x[2 * q + 1][0], first), x0, x1);
             o[0][q] = hmul2_u32(x0, d);
             o[1][q] = hmul2_u32(x1, d);
             if (kDims == 4) {
-              codes_to_h2(prmt(x[2 * q][0], x[2 * q + 1][0], 0x7362), x0, x1);
+              codes_to_h2(prmt(x[2 * q][0], x[2 * q + 1][0], second), x0, x1);
               o[2 % kDims][q] = hmul2_u32(x0, d);
               o[3 % kDims][q] = hmul2_u32(x1, d);
             }
@@ -411,7 +414,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         }
 #pragma unroll
         for (int e = 0; e < kDims; ++e)
-          sts128(dst + sw128_off(lane * kDims + e, 2 * (w & 3) + half), o[e][0], o[e][1], o[e][2], o[e][3]);
+          sts128(dst + sw128_off(row_of(e), 2 * (w & 3) + half), o[e][0], o[e][1], o[e][2], o[e][3]);
       }
     };
     bool go = true;
@@ -569,13 +572,15 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         }
         if (i < tiles) {
           float sum = 0.f, sum2 = 0.f;
+          // P at most 2^14, the power inside the exponent (its rounding there costs 2^-21 of a weight at most)
+          const float up14 = 14.f - zero;
 #pragma unroll 1
           for (int j = 0; j < 64; j += 16) {
             float x[16];
             uint32_t w[16];
             tmem_ld16(s + j, x);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = exp2_approx(fmaf(x[e], fac, -zero)) * 16384.f;
+            for (int e = 0; e < 16; ++e) x[e] = exp2_approx(fmaf(x[e], fac, up14));
             if (masked) {
               const int l0 = limit(j);
 #pragma unroll
