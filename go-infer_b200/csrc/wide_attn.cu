@@ -658,9 +658,12 @@ bool prepare_wide() {
 
 namespace paged {
 
-// From 96 rows on: 4 sequences of 8000 positions, 8 kv heads of 128, Q8_0, take 63 / 65 / 72 / 107 us here with
-// 64 / 96 / 128 / 256 rows per unit, and 58 / 65 / 131 / 211 us in units of at most 32 rows (paged_attn.cu).
-bool wide_ok(int head_dim, int rows) { return (head_dim == 64 || head_dim == 128) && rows >= 96; }
+// Head dim 128 from 48 rows on: 4 sequences of 8000 positions, 8 kv heads, Q8_0, take 55 / 56 / 59 / 98 us here
+// with 48 / 64 / 96 / 256 rows per unit, and 63 / 58 / 65 / 211 us in units of at most 32 rows (paged_attn.cu); a
+// prefix of 8192 under 48 / 64 sequences 35 / 39 and 41 / 45 us.  Sequences of 500 positions lose up to 2 us by it
+// (48 rows: 19.9 against 18.2).  Head dim 64, half the work per tile, from 64 rows on: 47 against 51 us with 64
+// rows, but 44 against 39 with 48.
+bool wide_ok(int head_dim, int rows) { return (head_dim == 128 && rows >= 48) || (head_dim == 64 && rows >= 64); }
 
 Rows wide_rows(int head_dim) { return {kRows, kTok, kRows * (head_dim + 2)}; }
 
