@@ -159,8 +159,9 @@ __global__ void __launch_bounds__(kWriteThreads) kv_write_kernel(
 
 // A CTA's tokens: 4-value chunks of their K and V rows, kReadAhead per thread
 // and step with all loads before the first store.  Whole tokens, in the order
-// of the output: 30011 tokens of 8 heads of 128 take 72 us (4.3 TB/s); with 16
-// tokens of one head in a row, which lie side by side in the cache, 79 us.
+// of the output: 30011 tokens of 8 heads of 128 take 54 us (5.8 TB/s).  It took
+// 72 us while indexes were divided by division, and 79 us in another order, 16
+// tokens of one head in a row, which lie side by side in the cache.
 template <int TYPE>
 __global__ void __launch_bounds__(kWriteThreads) kv_read_kernel(KvCache c, float* __restrict__ k,
                                                                 float* __restrict__ v,
