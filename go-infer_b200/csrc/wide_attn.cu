@@ -241,6 +241,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
     bool ok = true;
     const uint32_t mine = lane == 0, tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
     while (ok && walk.next(c, p, group, &u)) {
+      if (!u.tiles) continue;  // no queries come: their writer may be at most one phase ahead
       if (!(ok = wait(q_full, unit_no & 1))) break;
       ++unit_no;
       // S of tile i goes before P V of tile i - 1, which waits for the softmax
@@ -468,8 +469,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
       if (tiles < 0) break;
       // queries: a power of two per row that puts the largest just under 2^14, then
       // high and low halves into tensor memory, the A operand of S
-      float fac;
-      {
+      float fac = 0.f;
+      if (tiles) {
         const int row = s_unit->row0 + r;
         const bool real = r < s_unit->n_rows;
         const float4* q = reinterpret_cast<const float4*>(

@@ -277,6 +277,15 @@ def test_attention_of_many_rows(kind, heads, kv, dim, lens, new, prefix):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_many_rows_that_see_nothing(kind, dim):
+    """Unit after unit without a tile, with one that has tiles among them, in the run of every CTA."""
+    n = 40
+    lens = [300 if b % 7 == 3 else 0 for b in range(n)]
+    AttnCase(35 + dim, kind, 8, 1, dim, 16, lens, [64] * n).run()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_attention_of_many_rows_skips_pages_outside_the_cache(kind):
     c = AttnCase(13, kind, 8, 2, 128, 16, [400, 133], [100, 20])
     c.table[0, [0, 9, 20]], c.table[1, 8] = [-1, c.cache.n_pages, 10 ** 9], -7
