@@ -424,7 +424,8 @@ int gi_rope_freqs(int scaling, uint32_t dim, double theta, double factor, double
  * strides count floats and are multiples of 4), k + t * k_stride and
  * v + t * v_stride; q_out is [n_tokens][n_heads][head_dim] and may not
  * overlap q.  slots[t] is where K and V go; a slot outside the cache (-1
- * for a padding token) is not written, and no slot may appear twice.  q may be
+ * for a padding token) is not written, and no slot may appear twice.  What is
+ * cached is finite: magnitudes end at 65504 and NaN becomes 0.  q may be
  * NULL (n_heads is then ignored); rope may be NULL: nothing turns, positions
  * is not read. */
 int gi_cuda_kv_write_dev(const gi_cuda_kv_cache_t* cache, const float* k, size_t k_stride, const float* v,
@@ -461,7 +462,8 @@ int64_t gi_cuda_attn_workspace(const gi_cuda_kv_cache_t* cache, const gi_cuda_at
  * in the cache already.  A token sees the prefix (prefix_pages; NULL when
  * prefix_len is 0) and its sequence's positions up to its own.  A row that sees
  * nothing is 0; rows of no sequence are left as they are.  Positions that a
- * sequence does not have are not read, whatever their pages hold.  out and the
+ * sequence does not have are not read, whatever their pages hold; those that
+ * it has hold finite values, as the writes keep them.  out and the
  * workspace may not overlap q or the cache. */
 int gi_cuda_attn_dev(const gi_cuda_kv_cache_t* cache, const gi_cuda_attn_t* attn, float* out, const float* q,
                      uint32_t n_seqs, uint32_t n_tokens, const int32_t* q_start, const int32_t* kv_len,
