@@ -27,8 +27,11 @@
 // P V of one tile starts from zero; the running sum over tiles is a float32
 // FMA in the softmax threads' registers, so rounding does not grow with the
 // length (the tensor cores cut their sums).
-// Every wait is bounded in time; on expiry the CTA sets *error, its roles
-// leave, the products in flight are awaited (again bounded), tensor memory is freed.
+// Every wait for a barrier in memory is bounded in time; on expiry the CTA sets
+// *error, its roles leave, the products in flight are awaited (again bounded),
+// tensor memory is freed.  The softmax warps also meet at a named barrier, which
+// cannot give up: there they vote, and leave all together or not at all, since
+// one warp's wait may expire in the moment in which another's is over.
 #include "common.cuh"
 #include "gemv.cuh"
 #include "paged.cuh"
@@ -112,6 +115,16 @@ GI_DEVINL void commit_by(uint32_t mine, uint32_t bar) {
 
 // Named barrier of the softmax warps.
 GI_DEVINL void soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kSoftWarps) : "memory"); }
+// The same with a vote: whether `ok` holds in every thread, the same answer for all.
+GI_DEVINL bool soft_vote(bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{ .reg .pred p, q; setp.ne.b32 p, %1, 0; bar.red.and.pred q, 1, %2, p; selp.u32 %0, 1, 0, q; }"
+      : "=r"(all)
+      : "r"((uint32_t)ok), "n"(32 * kSoftWarps)
+      : "memory");
+  return all != 0;
+}
 
 // A unit of this CTA's run.
 struct Unit {
@@ -515,7 +528,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
       float o[kOut], m = -INFINITY, l = 0.f, alpha = 0.f;
 #pragma unroll
       for (int i = 0; i < kOut; ++i) o[i] = 0.f;
-      for (int i = 0; i <= tiles && ok && tiles; ++i) {
+      // A wait that gave up is taken to the next vote: no warp leaves on its own, and
+      // until then it touches neither tensor memory nor the barriers.
+      for (int i = 0; i <= tiles && tiles; ++i) {
         const int n_i = tile_no + i, p0 = i * kTok + 64 * half;
         const uint32_t s = s_col(n_i & 1) + lanes + 64 * half;
         uint32_t bad = 0;
@@ -525,13 +540,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         auto limit = [&](int j) { return (bad >> (8 * (j >> 4))) & 1 ? 0 : seen - p0 - j; };
         if (i < tiles) {
           const int n = n_i;
-          if (!(ok = wait(s_full(n & 1), phase(n)))) break;
+          ok = ok && wait(s_full(n & 1), phase(n));
           tc_fence_after();
           bad = *reinterpret_cast<const volatile uint32_t*>(s_bad + 8 * (n & 3) + 4 * half);
           masked = p0 + 64 > seen_first || bad;  // uniform in the warp
           float top = -INFINITY;
 #pragma unroll 1
-          for (int j = 0; j < 64; j += 32) {
+          for (int j = ok ? 0 : 64; j < 64; j += 32) {
             float x[32];
             tmem_ld32(s + j, x);
             if (masked) {
@@ -551,7 +566,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
             top = fmaxf(top, t2);
           }
           s_max[((n & 1) * 2 + half) * kRows + r] = top;
-          soft_sync();
+          if (!(ok = soft_vote(ok))) break;
           top = fmaxf(top, s_max[((n & 1) * 2 + (half ^ 1)) * kRows + r]);
           const float mn = top == -INFINITY ? m : fmaxf(m, top * fac);
           zero = mn == -INFINITY ? 0.f : mn;
@@ -560,7 +575,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         }
         if (i > 0) {  // o = o alpha + P V of the tile before, before this tile's P lets the next one begin
           const int n = tile_no + i - 1;
-          if (!(ok = wait(o_full(n & 1), phase(n)))) break;
+          ok = ok && wait(o_full(n & 1), phase(n));
+          if (!ok) continue;
           tc_fence_after();
 #pragma unroll
           for (int d = 0; d < kOut; d += 32) {
@@ -607,11 +623,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         alpha = alpha_n;
       }
       tile_no += tiles;
-      if (!ok) break;
 
       // ---- the row: finished, its sums, or a part ----
       s_ml[half * kRows + r] = make_float2(m, l);
-      soft_sync();
+      if (!(ok = soft_vote(ok))) break;
       const float sum = l + s_ml[(half ^ 1) * kRows + r].y;
       const int row = s_unit->row0 + r;
       const bool real = r < s_unit->n_rows;
