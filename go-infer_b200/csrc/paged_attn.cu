@@ -512,6 +512,8 @@ __global__ void __launch_bounds__(kMergeThreads) attn_merge_kernel(KvCache c, Pa
     const Pass& p = k ? own : pre;
     const Rows& w = k ? ro : rp;
     src[k].s = seq_of(p, k ? b : 0, c.page_shift);
+    // Only a q_start that does not ascend leaves a token outside the prefix pass's rows: it has no place on that line.
+    if (k == 0 && (token < src[k].s.start || token - src[k].s.start >= src[k].s.fresh)) return;
     src[k].n = span_of(p, src[k].s, group, c.n_kv_heads, w.rows, w.tt);
     src[k].chunk = p.line[0];
     src[k].line = p.line[1 + (k ? b : 0)];

@@ -457,13 +457,14 @@ int64_t gi_cuda_attn_workspace(const gi_cuda_kv_cache_t* cache, const gi_cuda_at
 /* Attention of a ragged batch over the cache, head h with kv head
  * h / (n_heads / n_kv_heads).  Sequence b's tokens are rows
  * q_start[b] .. q_start[b + 1] - 1 of q and out ([n_tokens][n_heads][head_dim],
- * q_start ascending; NULL: row b alone, n_tokens = n_seqs); they are the last
- * of its kv_len[b] positions, which lie in pages[b * pages_stride ...] and are
- * in the cache already.  A token sees the prefix (prefix_pages; NULL when
- * prefix_len is 0) and its sequence's positions up to its own.  A row that sees
- * nothing is 0; rows of no sequence are left as they are.  Positions that a
- * sequence does not have are not read, whatever their pages hold; those that
- * it has hold finite values, as the writes keep them.  out and the
+ * q_start ascending, else what out then holds is not defined; NULL: row b
+ * alone, n_tokens = n_seqs); they are the last of its kv_len[b] positions,
+ * which lie in pages[b * pages_stride ...] and are in the cache already.  A
+ * token sees the prefix (prefix_pages; NULL when prefix_len is 0) and its
+ * sequence's positions up to its own.  A row that sees nothing is 0; rows of
+ * no sequence are left as they are.  Positions that a sequence does not have
+ * are not read, whatever their pages hold; those that it has hold finite
+ * values, as the writes keep them.  out and the
  * workspace may not overlap q or the cache. */
 int gi_cuda_attn_dev(const gi_cuda_kv_cache_t* cache, const gi_cuda_attn_t* attn, float* out, const float* q,
                      uint32_t n_seqs, uint32_t n_tokens, const int32_t* q_start, const int32_t* kv_len,

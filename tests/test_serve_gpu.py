@@ -346,6 +346,27 @@ def test_attention_skips_prefix_pages_outside_the_cache(kind, new):
     c.run()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("start", [[500, 0, 600], [0, 600, 300], [-40, 700, 20], [600, 600, 0]])
+def test_attention_with_a_q_start_that_does_not_ascend(kind, start):
+    """What the rows hold is not defined, but nothing beside them is touched, and the next call is right."""
+    c = AttnCase(36, kind, 4, 1, 128, 16, [540, 160], [500, 100], prefix=300)
+    n, guard = c.ws.numel(), 1 << 16
+    around = torch.full((n + 2 * guard,), 85, dtype=torch.uint8, device="cuda:0")
+    out = torch.full((c.tokens + 64, 4, 128), 5.0, device="cuda:0")
+    c.ws, c.out = around[guard:guard + n], out[32:32 + c.tokens]
+    good = c.d["start"].clone()
+    c.d["start"].copy_(dev(start, np.int32))
+    torch.cuda.synchronize()
+    c.call()
+    c.stream.synchronize()
+    assert (around[:guard] == 85).all() and (around[guard + n:] == 85).all()
+    assert (out[:32] == 5).all() and (out[32 + c.tokens:] == 5).all()
+    c.d["start"].copy_(good)
+    torch.cuda.synchronize()
+    c.run()
+
+
 def test_attention_large_scores_and_flat_rows():
     """Scores of several hundred (one weight takes all) and a q of zeros (all weights equal)."""
     c = AttnCase(8, G.TYPE_F16, 4, 2, 128, 16, [70, 300])
