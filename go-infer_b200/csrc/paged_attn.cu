@@ -6,7 +6,9 @@
 // Sequence b has len = kv_len[b] cached positions in its own pages, the last
 // `new` of which are its tokens q_start[b] .. q_start[b+1] - 1 of this call.
 // Token j of them sees the whole prefix and its own positions below
-// len - new + j + 1; with nothing to see its row is 0.
+// len - new + j + 1; with nothing to see its row is 0.  A row of q that is not
+// finite becomes NaN: its scores are, no maximum takes them up (m stays -inf),
+// but its sums are NaN, and they are joined whatever m is.
 //
 // out = sum_t p_t v_t / sum_t p_t, p_t = 2^(s_t - m), s_t = log2(e) scale q.k_t,
 // in one pass over the positions with the running maximum m: a tile of
@@ -443,11 +445,12 @@ __global__ void __launch_bounds__(kAttnThreads, MINB) attn_tiles_kernel(KvCache 
       float top = -INFINITY, sum = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w * T::kRows + r].x);
+      const float base = top == -INFINITY ? 0.f : top;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float2 e = s_ml[w * T::kRows + r];
-        sum += top == -INFINITY ? 0.f : e.y * exp2_approx(e.x - top);
+        sum += e.y * exp2_approx(e.x - base);
         const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(sm) +
                                                           ((size_t)w * T::kRows + r) * HD + d);
         x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
@@ -558,14 +561,14 @@ __global__ void __launch_bounds__(kMergeThreads) attn_merge_kernel(KvCache c, Pa
         float mn = top;
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) mn = fmaxf(mn, e[a].x);
-        if (mn == -INFINITY) continue;
-        const float f0 = exp2_approx(top - mn);
+        const float base = mn == -INFINITY ? 0.f : mn;  // nothing seen, or not a number
+        const float f0 = exp2_approx(top - base);
         x.x *= f0, x.y *= f0, x.z *= f0, x.w *= f0;
         sum *= f0;
         top = mn;
 #pragma unroll
         for (int a = 0; a < kAhead; ++a) {
-          const float f = exp2_approx(e[a].x - mn);
+          const float f = exp2_approx(e[a].x - base);
           x.x = fmaf(y[a].x, f, x.x), x.y = fmaf(y[a].y, f, x.y);
           x.z = fmaf(y[a].z, f, x.z), x.w = fmaf(y[a].w, f, x.w);
           sum = fmaf(e[a].y, f, sum);

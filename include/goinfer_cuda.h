@@ -461,8 +461,8 @@ int64_t gi_cuda_attn_workspace(const gi_cuda_kv_cache_t* cache, const gi_cuda_at
  * alone, n_tokens = n_seqs); they are the last of its kv_len[b] positions,
  * which lie in pages[b * pages_stride ...] and are in the cache already.  A
  * token sees the prefix (prefix_pages; NULL when prefix_len is 0) and its
- * sequence's positions up to its own.  A row that sees nothing is 0; rows of
- * no sequence are left as they are.  Positions that a sequence does not have
+ * sequence's positions up to its own.  A row that sees nothing is 0, one whose
+ * q is not finite NaN; rows of no sequence are left as they are.  Positions that a sequence does not have
  * are not read, whatever their pages hold; those that it has hold finite
  * values, as the writes keep them.  out and the
  * workspace may not overlap q or the cache. */

@@ -377,6 +377,33 @@ def test_attention_large_scores_and_flat_rows():
     c.run()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("lens,new,prefix", [
+    ([30, 50, 9], [1, 1, 1], 0), ([5000, 40], [1, 1], 0), ([30, 3000], [1, 1], 70),         # whole units, cut ones, a prefix
+    ([70, 300], [60, 64], 0), ([3000, 200], [64, 60], 0), ([900, 60], [64, 50], 500), ([3, 9] * 30, [1] * 60, 700)])
+def test_attention_of_a_query_that_is_not_finite(kind, bad, lens, new, prefix):
+    """Its row is not a number wherever the line of tiles is cut; every other row is as it would be without it."""
+    c = AttnCase(37, kind, 8, 2, 128, 16, lens, new, prefix=prefix)
+    rows = [(0, 1), (c.tokens - 1, 7), (c.tokens // 2, 4)]
+    for t, h in rows:
+        c.q[t, h, 5] = bad
+        c.q[t, h, 6] = -c.q[t, h, 5]  # with an infinity no score is a number either
+    c.d["q"].copy_(dev(c.q))
+    torch.cuda.synchronize()
+    c.call()
+    c.stream.synchronize()
+    got = c.out.cpu().numpy()
+    for t, h in rows:
+        assert np.isnan(got[t, h]).all()
+    want, bound = attention(c.cache, np.nan_to_num(c.q, nan=0, posinf=0, neginf=0), c.start, c.lens, c.table, c.scale,
+                            c.prefix_pages, prefix, out=np.full(got.shape, 5.0))
+    ok = np.ones(got.shape[:2], bool)
+    for t, h in rows:
+        ok[t, h] = False
+    assert (np.abs(got - want).max(-1)[ok] <= bound[ok]).all()
+
+
 @pytest.mark.parametrize("size", [1e-30, 1e-3, 1e4])
 @pytest.mark.parametrize("kind", KINDS)
 def test_attention_of_any_magnitude_of_q_and_v(kind, size):
