@@ -404,6 +404,46 @@ def test_attention_of_a_query_that_is_not_finite(kind, bad, lens, new, prefix):
     assert (np.abs(got - want).max(-1)[ok] <= bound[ok]).all()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("seqs", [1, 40])
+def test_attention_of_many_rows_keeps_far_scores_apart(kind, dim, seqs):
+    """Scores near -757 * 60, exact in float32, whose maximum rises from tile to tile; V is 1 in even tiles and -1 in
+    odd ones, so a weight's error that differs between tiles shows in full.  The maxima are just above -65536 in
+    binades, where a sum with a few more binades would have coarser steps than they.
+
+    With exact scores a weight is off by its exponent's factor (2^-23 of at most 4 binades of distance), the
+    exponent's last rounding (2^-22 of a binade), exp2 (2^-22), the split (2^-22) and, in up to 11 tiles, the
+    factors between maxima (2^-22 each); sums of 64 to 128 values round or cut at 2^-23 a step, once in the sums of
+    weights and once in P V: below 2^-16 of max|V| in all, while half a step beyond 65536 is 2^-8."""
+    n, new = 1400, 16
+    c = AttnCase(38, kind, 8, 2, dim, 16, [n] * seqs, [new] * seqs, scale=1.0)
+    rng = np.random.default_rng(39)
+    k1 = np.array([rng.integers(-8, p // 128 + 1) for p in range(n)])
+    sign = np.where(np.arange(n) // 128 % 2, -1.0, 1.0)
+    c.cache.k[:], c.cache.v[:] = 0, 0
+    for x in (c.cache.ks, c.cache.vs):
+        if x is not None:
+            x[:] = 1
+    p = np.arange(n)
+    for b in range(seqs):
+        page, o = c.table[b, p // 16], p % 16
+        c.cache.k[page, :, o, 0] = -60
+        c.cache.k[page, :, o, 1] = k1[:, None]
+        c.cache.v[page, :, o] = sign[:, None, None]
+    c.q[:] = 0
+    c.q[..., 0] = 757
+    c.q[..., 1] = 0.125
+    c.data.copy_(dev(c.cache.data)), c.d["q"].copy_(dev(c.q))
+    torch.cuda.synchronize()
+    c.call()
+    c.stream.synchronize()
+    w = np.exp(k1 / 8)
+    want = (np.cumsum(w * sign) / np.cumsum(w))[n - new:]
+    got = c.out.cpu().numpy().reshape(seqs, new, 8, dim)
+    assert np.abs(got - want[:, None, None]).max() <= 2.0 ** -16
+
+
 @pytest.mark.parametrize("size", [1e-30, 1e-3, 1e4])
 @pytest.mark.parametrize("kind", KINDS)
 def test_attention_of_any_magnitude_of_q_and_v(kind, size):
