@@ -449,6 +449,8 @@ int capi_ready(CapiCtx* c) {
 
 int capi_fail(int code, const char* what, cudaError_t e) { return fail(code, what, e); }
 
+int capi_device_error() { return check_device_error(); }
+
 int model_generate(ModelHandle* h, const int32_t* tokens, uint32_t n_tokens, uint32_t start_pos, uint32_t n_gen,
                    const std::function<int(int, cudaStream_t)>& begin, uint32_t* out_tokens, float* out_logits,
                    float* decode_ms) {

@@ -39,6 +39,9 @@ struct ModelHandle {
 int model_generate(ModelHandle* h, const int32_t* tokens, uint32_t n_tokens, uint32_t start_pos, uint32_t n_gen,
                    const std::function<int(int, cudaStream_t)>& begin, uint32_t* out_tokens, float* out_logits,
                    float* decode_ms);
+// -6, with its text set, when a bounded wait has given up since this was last
+// asked (a look at host memory; mutex held).
+int capi_device_error();
 // Sets gi_cuda_last_error's text and returns `code`.
 int capi_fail(int code, const char* what, cudaError_t e = cudaSuccess);
 

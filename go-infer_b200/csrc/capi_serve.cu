@@ -83,6 +83,13 @@ int serve_ready(gi::CapiCtx* ctx) {
   return 0;
 }
 
+// The same for a call that launches.  What it launches ends after it has returned, so a wait that gave up there is
+// reported by the next call: programs that make no others would not learn of it.
+int launch_ready(gi::CapiCtx* ctx) {
+  if (int rc = serve_ready(ctx)) return rc;
+  return gi::capi_device_error();
+}
+
 }  // namespace
 
 extern "C" {
@@ -131,7 +138,7 @@ int gi_cuda_kv_write_dev(const gi_cuda_kv_cache_t* cache, const float* k, size_t
   }
   std::lock_guard<std::mutex> lk(gi::capi_mutex());
   gi::CapiCtx ctx;
-  if (int rc = serve_ready(&ctx)) return rc;
+  if (int rc = launch_ready(&ctx)) return rc;
   if (!n_tokens) return 0;
   GI_CUDA_TRY(gi::kv_write_launch(c, k, k_stride, v, v_stride, slots, (int)n_tokens, q, q_stride, q_out, (int)n_heads,
                                   positions, r, ctx.sm_count, stream_of(ctx, stream)),
@@ -148,7 +155,7 @@ int gi_cuda_kv_read_dev(const gi_cuda_kv_cache_t* cache, float* k, float* v, con
   if (misaligned(k) || misaligned(v)) return fail(-4, "rows must be 16-byte aligned");
   std::lock_guard<std::mutex> lk(gi::capi_mutex());
   gi::CapiCtx ctx;
-  if (int rc = serve_ready(&ctx)) return rc;
+  if (int rc = launch_ready(&ctx)) return rc;
   if (!n_tokens) return 0;
   GI_CUDA_TRY(gi::kv_read_launch(c, k, v, slots, (int)n_tokens, ctx.sm_count, stream_of(ctx, stream)), "cache read");
   return 0;
@@ -181,7 +188,7 @@ int gi_cuda_attn_dev(const gi_cuda_kv_cache_t* cache, const gi_cuda_attn_t* attn
   if (misaligned(out) || misaligned(q)) return fail(-4, "rows must be 16-byte aligned");
   std::lock_guard<std::mutex> lk(gi::capi_mutex());
   gi::CapiCtx ctx;
-  if (int rc = serve_ready(&ctx)) return rc;
+  if (int rc = launch_ready(&ctx)) return rc;
   const size_t need = gi::attn_workspace(c, a, ctx.sm_count);
   if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255)))
     return fail(-4, "workspace missing, too small or not 256-byte aligned");
@@ -221,7 +228,7 @@ int gi_cuda_sample_dev(int32_t* ids, float* prob, const float* logits, size_t lo
   p.min_p = min_p;
   std::lock_guard<std::mutex> lk(gi::capi_mutex());
   gi::CapiCtx ctx;
-  if (int rc = serve_ready(&ctx)) return rc;
+  if (int rc = launch_ready(&ctx)) return rc;
   if (!rows) return 0;
   GI_CUDA_TRY(gi::sample_launch(p, ctx.sm_count, stream_of(ctx, stream)), "sampling");
   return 0;

@@ -372,7 +372,10 @@ int gi_synth_weights(gi_cuda_buffer_t buf, int quant_type, uint64_t seed, float 
  * device and can be captured; lengths, positions, slots and pages are read on
  * the device when the call runs, so a captured call follows them.  Indexes
  * that lie outside their range are never followed: such a slot is skipped,
- * the positions of such a page are not seen. */
+ * the positions of such a page are not seen.  A kernel's wait that gives up
+ * (GI_ERR_TIMEOUT; the output is then not valid) shows after its call has
+ * returned: the next of these calls returns it and launches nothing, or the
+ * next call that waits for the device does. */
 
 /* A layer's cache: n_pages pages of page_size positions (a power of two from
  * 16 to 65536) of n_kv_heads heads of head_dim values (a multiple of 32 up to

@@ -35,3 +35,21 @@ def test_batch_mode_on_fake_runtime(tmp_path):
                     str(capi), "-o", str(exe), "-lpthread"], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stdout[-4000:] + r.stderr[-4000:]
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_serving_calls_on_fake_runtime(tmp_path):
+    """capi_serve.cu beside capi.cu: what the serving calls report and refuse before they launch."""
+    csrc = os.path.join(ROOT, "go-infer_b200", "csrc")
+    inc = ["-I", FAKE, "-I", csrc, "-I", os.path.join(ROOT, "include")]
+    flags = ["-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-fno-sanitize-recover=undefined"]
+    objs = []
+    for name in ("capi", "capi_serve"):
+        objs.append(str(tmp_path / (name + ".o")))
+        subprocess.run(["g++", *flags, "-x", "c++", *inc, "-c", os.path.join(csrc, name + ".cu"), "-o", objs[-1]],
+                       check=True)
+    exe = tmp_path / "serve_driver"
+    subprocess.run(["g++", *flags, *inc, os.path.join(FAKE, "fake_device.cc"), os.path.join(FAKE, "serve_driver.cc"),
+                    *objs, "-o", str(exe), "-lpthread"], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("ok"), r.stdout[-4000:] + r.stderr[-4000:]
