@@ -21,6 +21,7 @@ int fail(int code, const char* what, cudaError_t e = cudaSuccess) { return gi::c
   } while (0)
 
 constexpr uint32_t kMaxServeHeads = 1024;
+constexpr uint32_t kMaxServeTokens = 1u << 30;  // the launches' sums of them and their blocks fit an int
 
 bool cache_shape_ok(const gi_cuda_kv_cache_t& c) {
   return (c.type == GI_TYPE_F16 || c.type == GI_TYPE_Q8_0) && c.n_pages && c.page_size >= 16 &&
@@ -120,7 +121,7 @@ int gi_cuda_kv_write_dev(const gi_cuda_kv_cache_t* cache, const float* k, size_t
   if (!k || !v || !slots || (q && !q_out)) return fail(-4, "null device pointer");
   if (!q) n_heads = 0;
   if (q && (!n_heads || n_heads > kMaxServeHeads)) return fail(-4, "n_heads out of range");
-  if (n_tokens > INT32_MAX) return fail(-4, "too many tokens");
+  if (n_tokens > kMaxServeTokens) return fail(-4, "too many tokens");
   if (misaligned(k) || misaligned(v) || misaligned(q) || misaligned(q_out) || k_stride % 4 || v_stride % 4 ||
       (q && q_stride % 4))
     return fail(-4, "rows must be 16-byte aligned");
@@ -151,7 +152,7 @@ int gi_cuda_kv_read_dev(const gi_cuda_kv_cache_t* cache, float* k, float* v, con
   gi::KvCache c;
   if (int rc = kv_cache_ref(cache, &c)) return rc;
   if (!k || !v || !slots) return fail(-4, "null device pointer");
-  if (n_tokens > INT32_MAX) return fail(-4, "too many tokens");
+  if (n_tokens > kMaxServeTokens) return fail(-4, "too many tokens");
   if (misaligned(k) || misaligned(v)) return fail(-4, "rows must be 16-byte aligned");
   std::lock_guard<std::mutex> lk(gi::capi_mutex());
   gi::CapiCtx ctx;

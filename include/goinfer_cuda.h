@@ -423,7 +423,7 @@ int gi_rope_freqs(int scaling, uint32_t dim, double theta, double factor, double
                   double* freqs, double* mscale);
 
 /* Rotates q into q_out and k into the cache, and writes v beside it, for
- * n_tokens tokens.  Token t's rows are q + t * q_stride (n_heads heads; the
+ * n_tokens tokens (up to 2^30).  Token t's rows are q + t * q_stride (n_heads heads; the
  * strides count floats and are multiples of 4), k + t * k_stride and
  * v + t * v_stride; q_out is [n_tokens][n_heads][head_dim] and may not
  * overlap q.  slots[t] is where K and V go; a slot outside the cache (-1

@@ -76,6 +76,14 @@ def test_read_refusals():
     refused(G.ERR_SHAPE, "aligned", G.kv_read_dev, cache(), A, A + 4, A, 1)
 
 
+def test_token_counts_that_are_refused():
+    """Up to 2^30 tokens: a launch adds blocks to them in 32 bits, and near 2^31 it divided by zero."""
+    c = cache()
+    for n in ((1 << 30) + 1, (1 << 31) - 1, 1 << 31, (1 << 32) - 1):
+        refused(G.ERR_SHAPE, "too many tokens", G.kv_write_dev, c, A, A, A, n)
+        refused(G.ERR_SHAPE, "too many tokens", G.kv_read_dev, c, A, A, A, n)
+
+
 def attention(c, **kw):
     d = {**dict(heads=4, max_tokens=8, max_q_len=4, scale=0.125, prefix_len=0), **kw}
     a = G.Attention.__new__(G.Attention)
