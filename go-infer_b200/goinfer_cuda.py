@@ -466,8 +466,9 @@ class KVCache:
         self._p = ctypes.addressof(self.desc)
 
     def close(self) -> None:
-        ReleaseBuffer(self.buf)
-        self.buf = None
+        if self.buf is not None:
+            ReleaseBuffer(self.buf)
+            self.desc.data, self.buf = None, None  # calls are refused from here on
 
 
 def rope_freqs(dim: int, theta: float, scaling: int = ROPE_NONE, factor: float = 1.0, low: float = 1.0,

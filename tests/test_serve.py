@@ -52,6 +52,18 @@ def test_cache_data_that_is_refused():
     refused(G.ERR_SHAPE, "256-byte", G.kv_read_dev, cache(data_ptr=A + 16), A, A, A, 1)
 
 
+def test_a_closed_cache_is_refused():
+    """Its buffer is gone: a call afterwards must not follow the address."""
+    c = G.KVCache(G.TYPE_F16, 4, 16, 2, 64, data_ptr=A, nbytes=1 << 20)
+    c.buf = G.Buffer(0, 1 << 20)  # as if the cache had made it
+    c.close()
+    refused(G.ERR_BUFFER, "cache data", G.kv_read_dev, c, A, A, A, 1)
+    c.close()
+    own = G.KVCache(G.TYPE_F16, 4, 16, 2, 64, data_ptr=A, nbytes=1 << 20)
+    own.close()  # the caller's memory stays the caller's
+    assert own.desc.data == A
+
+
 def test_write_refusals():
     c, w = cache(), G.kv_write_dev
     rope = G.Rope(64, A)
