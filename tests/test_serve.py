@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 import goinfer_cuda as G
+import _precision
 from _serve import Cache, sample
 
 CACHE = dict(type=G.TYPE_Q8_0, n_pages=4, page_size=16, n_kv_heads=2, head_dim=64)
@@ -181,3 +182,13 @@ def test_model_refusals_without_a_model():
     toks, out = (G.ctypes.c_int32 * 1)(1), (G.ctypes.c_uint32 * 1)()
     u = (G.ctypes.c_float * 1)(0.5)
     assert lib.gi_cuda_model_generate_sampled(None, toks, 1, 0, 1, 1.0, 0, 1.0, 0.0, u, out, None, None) == G.ERR_SHAPE
+
+
+@pytest.mark.parametrize("kind", _precision.KINDS)
+@pytest.mark.parametrize("shape", _precision.SHAPES)
+def test_one_half_of_an_operand_misses_the_precision(kind, shape):
+    """What the GPU's test of these cases would see if q, or the weights, were held in one half."""
+    c = _precision.Case(kind, *shape)
+    want, tol = c.out(), c.tolerance()
+    assert _precision.off(c.out(q=_precision.half), want) > 2 * tol
+    assert _precision.off(c.out(p=_precision.half), want) > 2 * tol

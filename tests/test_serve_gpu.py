@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 import goinfer_cuda as G
+import _precision
 from _serve import Cache, attention, sample
 
 pytestmark = pytest.mark.gpu
@@ -479,6 +480,25 @@ def test_attention_calls_repeat_bit_for_bit_and_side_by_side(kind):
     graph.replay()
     torch.cuda.synchronize()
     a.check(lens=[10, 650, 3])
+
+
+@pytest.mark.parametrize("kind", _precision.KINDS)
+@pytest.mark.parametrize("shape", _precision.SHAPES)
+def test_attention_holds_its_operands_to_22_bits(kind, shape):
+    """The tolerance is one that a q or a weight in a single half fails (test_serve.py), in every kernel."""
+    x = _precision.Case(kind, *shape)
+    data, gc = on_gpu(x.cache)
+    q, st = dev(x.q), torch.cuda.Stream()
+    out = torch.zeros(x.new, x.heads, x.dim, device="cuda:0")
+    att = G.Attention(gc, heads=x.heads, max_tokens=x.new, max_q_len=x.new, scale=x.scale)
+    ws = torch.empty(max(att.workspace_bytes, 1), dtype=torch.uint8, device="cuda:0")
+    lens, start = dev([x.n], np.int32), dev([0, x.new], np.int32)
+    table = dev(np.arange(x.cache.n_pages), np.int32)
+    torch.cuda.synchronize()
+    att(out.data_ptr(), q.data_ptr(), 1, x.new, lens.data_ptr(), table.data_ptr(), x.cache.n_pages, ws.data_ptr(), ws.numel(),
+        q_start_ptr=start.data_ptr(), stream=st.cuda_stream)
+    st.synchronize()
+    assert _precision.off(out.cpu().numpy(), x.out()) <= x.tolerance()
 
 
 # ---- sampling ----------------------------------------------------------------------
