@@ -6,6 +6,7 @@ import pytest
 
 import goinfer_cuda as G
 import _precision
+from _line import Line
 from _serve import Cache, attention, sample
 
 pytestmark = pytest.mark.gpu
@@ -499,6 +500,21 @@ def test_attention_holds_its_operands_to_22_bits(kind, shape):
         q_start_ptr=start.data_ptr(), stream=st.cuda_stream)
     st.synchronize()
     assert _precision.off(out.cpu().numpy(), x.out()) <= x.tolerance()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_many_rows_where_units_without_tiles_alternate(kind, dim):
+    """Runs of ten and more units, those that see nothing between those that have tiles, in orders of every kind:
+    the roles of a CTA skip the first and keep their phases through the others."""
+    rng = np.random.default_rng(41)
+    lens = [int(rng.choice([0, 0, 0, 40, 128, 129, 300])) for _ in range(1800)]
+    c = AttnCase(42 + dim, kind, 4, 1, dim, 16, lens, [2] * len(lens), hint=16)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    line = Line(c.start.tolist(), lens, c.tokens, 4, 1, 128, 128, 2, sms, 1)
+    runs = ["".join("T" if u[-1] else "E" for u in line.units(cta)) for cta in range(sms)]
+    assert sum(len(r) >= 10 for r in runs) > sms // 2 and any("EEETE" in r for r in runs) and any("TETTE" in r for r in runs)
+    c.run()
 
 
 # ---- sampling ----------------------------------------------------------------------
