@@ -517,6 +517,119 @@ def test_attention_of_many_rows_where_units_without_tiles_alternate(kind, dim):
     c.run()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("size", [1e-30, 1e-3, 1e4])
+def test_attention_of_many_rows_of_any_magnitude(kind, dim, size):
+    c = AttnCase(43, kind, 8, 2, dim, 16, [400, 90], [70, 60], prefix=50)
+    c.q *= size
+    c.q[::5] = 0  # all weights equal
+    c.q[1] *= 300  # scores of several hundred at size 1 and above: one weight takes all
+    c.d["q"].copy_(dev(c.q))
+    torch.cuda.synchronize()
+    c.run()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv,lens,new,prefix", [
+    (3, 1, [150, 70], [97, 2], 0), (6, 2, [40, 200, 9], [12, 1, 3], 0), (4, 4, [0, 30, 90], None, 170), (12, 1, [60, 33], [9, 4], 250)])
+def test_attention_of_head_dim_96(kind, heads, kv, lens, new, prefix):
+    AttnCase(44 + heads, kind, heads, kv, 96, 16, lens, new, prefix=prefix, pad=2).run()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("lens,new,prefix", [([20011, 9000], None, 0), ([30, 700], None, 12345), ([12007], [50], 0),
+                                             ([40] * 50, None, 9001)])
+def test_attention_over_long_contexts(kind, lens, new, prefix):
+    AttnCase(45, kind, 4, 2, 64, 64, lens, new, prefix=prefix).run()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_cache_whose_offsets_pass_32_bits(kind):
+    """The highest pages of a cache of 10 GB and more answer as a small cache's: what is written there, read back and
+    attended over, by single tokens and by chunks."""
+    kv, dim, page, n, heads = 8, 128, 64, 200, 16
+    n_pages = (1 << 32) // (kv * dim * page) + 8  # values past 2^32
+    rng = np.random.default_rng(46)
+    kvs = dev(rng.normal(size=(2, n, kv, dim)), np.float32)
+    q = dev(rng.normal(size=(64, heads, dim)), np.float32)
+    st = torch.cuda.Stream()
+    got = []
+    for pages in (n_pages, 8):
+        size = int(G.load_library().gi_kv_cache_bytes(kind, pages, page, kv, dim))
+        data = torch.empty(size, dtype=torch.uint8, device="cuda:0")
+        gc = G.KVCache(kind, pages, page, kv, dim, data_ptr=data.data_ptr(), nbytes=size)
+        table = pages - 1 - np.array([0, 2, 5, 3])
+        p = np.arange(n)
+        slots = dev(table[p // page] * page + p % page, np.int32)
+        back_k, back_v = torch.zeros(n, kv, dim, device="cuda:0"), torch.zeros(n, kv, dim, device="cuda:0")
+        table, lens = dev(table, np.int32), dev([n], np.int32)
+        torch.cuda.synchronize()
+        G.kv_write_dev(gc, kvs[0].data_ptr(), kvs[1].data_ptr(), slots.data_ptr(), n, stream=st.cuda_stream)
+        G.kv_read_dev(gc, back_k.data_ptr(), back_v.data_ptr(), slots.data_ptr(), n, stream=st.cuda_stream)
+        outs = [back_k, back_v]
+        for new in (1, 8, 64):
+            att = G.Attention(gc, heads=heads, max_tokens=new, max_q_len=new, scale=dim ** -0.5)
+            ws = torch.empty(att.workspace_bytes, dtype=torch.uint8, device="cuda:0")
+            start, out = dev([0, new], np.int32), torch.zeros(new, heads, dim, device="cuda:0")
+            torch.cuda.synchronize()
+            att(out.data_ptr(), q.data_ptr(), 1, new, lens.data_ptr(), table.data_ptr(), 4, ws.data_ptr(), ws.numel(),
+                q_start_ptr=start.data_ptr(), stream=st.cuda_stream)
+            st.synchronize()
+            outs.append(out)
+        got.append([x.cpu().numpy() for x in outs])
+        del data, gc, ws
+        torch.cuda.empty_cache()
+    for x, y in zip(*got):
+        assert np.array_equal(x, y) and np.abs(x).max() > 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("lens,new,prefix,other", [
+    ([30, 200, 90] * 17, [1] * 51, 700, [0, 17, 90] * 17),   # a prefix in units of 128 rows, single tokens beside it
+    ([300, 90], [70, 40], 0, [280, 75]), ([300, 90], [70, 40], 400, [299, 40])])
+def test_a_captured_call_of_many_rows_follows_its_lengths(kind, lens, new, prefix, other):
+    c = AttnCase(47, kind, 8, 2, 128, 16, lens, new, prefix=prefix)
+    first = c.run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=c.stream):
+        c.call()
+        c.call()
+    for now in (other, lens):
+        c.d["len"].copy_(dev(now, np.int32))
+        c.out.fill_(5.0)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            graph.replay()
+        torch.cuda.synchronize()
+        got = c.check(lens=now)
+    assert np.array_equal(got, first)
+
+
+def test_the_calls_allocate_nothing():
+    """Free device memory is the same after a first and after many of the calls."""
+    c = AttnCase(48, G.TYPE_Q8_0, 8, 2, 128, 16, [300, 90], [70, 1], prefix=100)
+    n, vocab = 40, 5000
+    k, v = torch.zeros(2, n, 2 * 128, device="cuda:0")
+    slots = torch.arange(n, dtype=torch.int32, device="cuda:0")
+    x, u = torch.zeros(3, vocab, device="cuda:0"), torch.zeros(3, device="cuda:0")
+    ids = torch.zeros(3, dtype=torch.int32, device="cuda:0")
+
+    def calls():
+        s = c.stream.cuda_stream
+        G.kv_read_dev(c.gc, k.data_ptr(), v.data_ptr(), slots.data_ptr(), n, stream=s)
+        G.kv_write_dev(c.gc, k.data_ptr(), v.data_ptr(), slots.data_ptr(), n, stream=s)
+        c.call()
+        G.sample_dev(ids.data_ptr(), x.data_ptr(), 3, vocab, u.data_ptr(), stream=s)
+        c.stream.synchronize()
+
+    calls()
+    free = torch.cuda.mem_get_info()[0]
+    for _ in range(20):
+        calls()
+    assert torch.cuda.mem_get_info()[0] == free
+
+
 # ---- sampling ----------------------------------------------------------------------
 
 def draw_ids(x, u, t=None, k=None, p=None, least=None, stride=0):
