@@ -21,6 +21,7 @@ int fail(int code, const char* what, cudaError_t e = cudaSuccess) { return gi::c
   } while (0)
 
 constexpr uint32_t kMaxServeHeads = 1024;
+constexpr uint32_t kMaxPositions = INT32_MAX - 255;  // of a sequence: the end of its last tile fits an int
 constexpr uint32_t kMaxServeTokens = 1u << 30;  // the launches' sums of them and their blocks fit an int
 
 bool cache_shape_ok(const gi_cuda_kv_cache_t& c) {
@@ -61,7 +62,8 @@ int attn_ref(const gi::KvCache& c, const gi_cuda_attn_t* d, gi::Attn* a) {
   if (!d->max_tokens || !d->max_q_len || d->max_q_len > d->max_tokens ||
       (uint64_t)d->max_tokens * d->n_heads > (1u << 30))
     return fail(-4, "max_tokens or max_q_len out of range");
-  if (d->prefix_len > (uint64_t)c.n_pages * c.page_size) return fail(-4, "prefix longer than the cache");
+  if (d->prefix_len > (uint64_t)c.n_pages * c.page_size || d->prefix_len > kMaxPositions)
+    return fail(-4, "prefix longer than the cache or 2^31 - 256 positions");
   a->n_heads = (int)d->n_heads;
   a->max_tokens = (int)d->max_tokens;
   a->max_q_len = (int)d->max_q_len;
@@ -185,7 +187,8 @@ int gi_cuda_attn_dev(const gi_cuda_kv_cache_t* cache, const gi_cuda_attn_t* attn
   if (n_tokens > attn->max_tokens) return fail(-4, "more tokens than the call was described for");
   if (n_seqs > attn->max_tokens) return fail(-4, "more sequences than max_tokens");
   if (!q_start && n_tokens != n_seqs) return fail(-4, "without q_start a sequence has one token");
-  if (!pages_stride || (uint64_t)pages_stride * c.page_size > INT32_MAX) return fail(-4, "pages_stride out of range");
+  if (!pages_stride || (uint64_t)pages_stride * c.page_size > kMaxPositions)
+    return fail(-4, "pages_stride out of range");
   if (misaligned(out) || misaligned(q)) return fail(-4, "rows must be 16-byte aligned");
   std::lock_guard<std::mutex> lk(gi::capi_mutex());
   gi::CapiCtx ctx;

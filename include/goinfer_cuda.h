@@ -462,8 +462,8 @@ int64_t gi_cuda_attn_workspace(const gi_cuda_kv_cache_t* cache, const gi_cuda_at
  * q_start[b] .. q_start[b + 1] - 1 of q and out ([n_tokens][n_heads][head_dim],
  * q_start ascending, else what out then holds is not defined; NULL: row b
  * alone, n_tokens = n_seqs); they are the last of its kv_len[b] positions,
- * which lie in pages[b * pages_stride ...] and are in the cache already.  A
- * token sees the prefix (prefix_pages; NULL when prefix_len is 0) and its
+ * which lie in pages[b * pages_stride ...] (up to 2^31 - 256 positions) and are
+ * in the cache already.  A token sees the prefix (prefix_pages; NULL when prefix_len is 0) and its
  * sequence's positions up to its own.  A row that sees nothing is 0, one whose
  * q is not finite NaN; rows of no sequence are left as they are.  Positions that a sequence does not have
  * are not read, whatever their pages hold; those that it has hold finite

@@ -127,6 +127,15 @@ def test_attention_refusals():
     refused(G.ERR_SHAPE, "aligned", a, A + 4, *args[1:], q_start_ptr=A)
 
 
+def test_lengths_whose_last_tile_would_pass_32_bits_are_refused():
+    """The kernels compare the end of a tile of up to 128 positions with the length in 32 bits."""
+    c, args = cache(), (A, A, 2, 8, A, A)
+    for stride in ((1 << 27) - 1, (1 << 27) - 15):  # pages of 16
+        refused(G.ERR_SHAPE, "pages_stride", attention(c), *args, stride, A, 1 << 30, q_start_ptr=A)
+    big = cache(n_pages=(1 << 27) - 1, nbytes=1 << 62)
+    refused(G.ERR_SHAPE, "prefix", attention(big, prefix_len=(1 << 31) - 17), *args, 3, A, 1 << 30, q_start_ptr=A)
+
+
 def test_sample_refusals():
     s = G.sample_dev
     refused(G.ERR_SHAPE, "vocab", s, A, A, 1, 0, A)
