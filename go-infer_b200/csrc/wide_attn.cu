@@ -48,7 +48,10 @@ constexpr int kRows = 128, kTok = 128;
 constexpr int kSoftWarps = 8, kKWarps = 4, kVWarps = 3, kLoadWarps = kKWarps + kVWarps;
 constexpr int kGroups = kTok / 16;  // of 16 positions, what a loading warp takes at a time
 constexpr int kWideThreads = 32 * (kSoftWarps + kLoadWarps + 1);
-constexpr int kWideCost = 2;  // tiles that a unit's start and end take
+// Tiles that a unit's start and end take.  With 0 / 1 / 2 / 4 / 8: 7 chunks of up to 512 on up to 4000 positions
+// 313 / 304 / 292 / 286 / 294 us, 60 of up to 64 on up to 2000 350 / 311 / 267 / 224 / 230 (32/8 heads of 128, Q8_0);
+// 200 of up to 32 on up to 500 245 / 236 / 212 / 208 / 221 (heads of 64, F16).
+constexpr int kWideCost = 4;
 constexpr int kTmem = 512;
 
 template <int HD, int TYPE>
@@ -675,10 +678,10 @@ bool prepare_wide() {
 
 namespace paged {
 
-// Head dim 128 from 48 rows on: 4 sequences of 8000 positions, 8 kv heads, Q8_0, take 55 / 56 / 59 / 98 us here
+// Head dim 128 from 48 rows on: 4 sequences of 8000 positions, 8 kv heads, Q8_0, take 54 / 55 / 56 / 96 us here
 // with 48 / 64 / 96 / 256 rows per unit, and 63 / 58 / 65 / 211 us in units of at most 32 rows (paged_attn.cu); a
 // prefix of 8192 under 48 / 64 sequences 35 / 39 and 41 / 45 us.  Sequences of 500 positions lose up to 2 us by it
-// (48 rows: 19.9 against 18.2).  Head dim 64, half the work per tile, from 64 rows on: 47 against 51 us with 64
+// (48 rows: 20.7 against 18.2).  Head dim 64, half the work per tile, from 64 rows on: 47 against 51 us with 64
 // rows, but 44 against 39 with 48.
 bool wide_ok(int head_dim, int rows) { return (head_dim == 128 && rows >= 48) || (head_dim == 64 && rows >= 64); }
 

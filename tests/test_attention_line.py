@@ -5,7 +5,7 @@ import pytest
 
 from _line import Line
 
-SHAPES = [(8, 16, 8, 444, 4), (32, 16, 8, 296, 4), (128, 128, 2, 148, 1)]  # rows, positions, unit cost, CTAs, least
+SHAPES = [(8, 16, 8, 444, 4), (32, 16, 8, 296, 4), (128, 128, 4, 148, 1)]  # rows, positions, unit cost, CTAs, least
 
 
 def owner(q_start, n_seqs, token):

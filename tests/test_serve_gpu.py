@@ -511,7 +511,7 @@ def test_attention_of_many_rows_where_units_without_tiles_alternate(kind, dim):
     lens = [int(rng.choice([0, 0, 0, 40, 128, 129, 300])) for _ in range(1800)]
     c = AttnCase(42 + dim, kind, 4, 1, dim, 16, lens, [2] * len(lens), hint=16)
     sms = torch.cuda.get_device_properties(0).multi_processor_count
-    line = Line(c.start.tolist(), lens, c.tokens, 4, 1, 128, 128, 2, sms, 1)
+    line = Line(c.start.tolist(), lens, c.tokens, 4, 1, 128, 128, 4, sms, 1)
     runs = ["".join("T" if u[-1] else "E" for u in line.units(cta)) for cta in range(sms)]
     assert sum(len(r) >= 10 for r in runs) > sms // 2 and any("EEETE" in r for r in runs) and any("TETTE" in r for r in runs)
     c.run()
