@@ -13,8 +13,8 @@
 // Q8_0: the framework's own block rule (quantize.cu, QuantizeQ8_0): 32
 // values, d = max|x| / 127 with its fp16 mantissa cut off, code =
 // round-half-away(clamp(x / d)).  A cached value is code * d rounded to half
-// precision (at most 2^-11 of the value, 1/16 of the half step of a code
-// near 127), because the attention's tensor-core products take halves; every
+// precision (at most 2^-11 of the value, 1/8 of the half step of a code near
+// 127), because the attention's tensor-core products take halves; every
 // reader uses that same value.  What would not be finite is not stored: NaN is
 // written as 0 and magnitudes end at 65504, so one bad token cannot reach
 // the other rows of a batch through P * V.

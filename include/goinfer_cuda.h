@@ -423,8 +423,8 @@ int gi_rope_freqs(int scaling, uint32_t dim, double theta, double factor, double
                   double* freqs, double* mscale);
 
 /* Rotates q into q_out and k into the cache, and writes v beside it, for
- * n_tokens tokens (up to 2^30).  Token t's rows are q + t * q_stride (n_heads heads; the
- * strides count floats and are multiples of 4), k + t * k_stride and
+ * n_tokens tokens (up to 2^30).  Token t's rows are q + t * q_stride (n_heads
+ * heads; the strides count floats and are multiples of 4), k + t * k_stride and
  * v + t * v_stride; q_out is [n_tokens][n_heads][head_dim] and may not
  * overlap q.  slots[t] is where K and V go; a slot outside the cache (-1
  * for a padding token) is not written, and no slot may appear twice.  What is
@@ -444,9 +444,11 @@ int gi_cuda_kv_read_dev(const gi_cuda_kv_cache_t* cache, float* k, float* v, con
 
 /* What an attention call's kernels and workspace are chosen by: n_heads query
  * heads (a multiple of the cache's n_kv_heads); at most max_tokens tokens and
- * as many sequences in a call, and max_q_len tokens of one sequence (the kernels are chosen by max_q_len; a longer
- * sequence is answered all the same, only slower); prefix_len positions that every sequence sees before its
- * own; scale on q.k. */
+ * as many sequences in a call, and max_q_len tokens of one sequence;
+ * prefix_len positions that every sequence sees before its own; scale on q.k.
+ * The kernels for all sequences of a call are chosen by max_q_len: a longer
+ * sequence is answered all the same, only slower, and single tokens beside
+ * long chunks are slower than in a call of their own. */
 typedef struct {
   uint32_t n_heads, max_tokens, max_q_len, prefix_len;
   float scale;
@@ -463,12 +465,14 @@ int64_t gi_cuda_attn_workspace(const gi_cuda_kv_cache_t* cache, const gi_cuda_at
  * q_start ascending, else what out then holds is not defined; NULL: row b
  * alone, n_tokens = n_seqs); they are the last of its kv_len[b] positions,
  * which lie in pages[b * pages_stride ...] (up to 2^31 - 256 positions) and are
- * in the cache already.  A token sees the prefix (prefix_pages; NULL when prefix_len is 0) and its
- * sequence's positions up to its own.  A row that sees nothing is 0, one whose
- * q is not finite NaN; rows of no sequence are left as they are.  Positions that a sequence does not have
- * are not read, whatever their pages hold; those that it has hold finite
- * values, as the writes keep them.  out and the
- * workspace may not overlap q or the cache. */
+ * in the cache already.  A token sees the prefix (prefix_pages; NULL when
+ * prefix_len is 0) and its sequence's positions up to its own.  A row that
+ * sees nothing is 0, one whose q is not finite NaN; rows of no sequence are
+ * left as they are.  Positions that a sequence does not have are not read,
+ * whatever their pages hold; those that it has hold finite values, as the
+ * writes keep them.  q and the softmax's weights enter the products with 22
+ * bits (two halves each), sums are float32.  out and the workspace may not
+ * overlap q or the cache. */
 int gi_cuda_attn_dev(const gi_cuda_kv_cache_t* cache, const gi_cuda_attn_t* attn, float* out, const float* q,
                      uint32_t n_seqs, uint32_t n_tokens, const int32_t* q_start, const int32_t* kv_len,
                      const int32_t* pages, uint32_t pages_stride, const int32_t* prefix_pages, void* workspace,
@@ -477,10 +481,10 @@ int gi_cuda_attn_dev(const gi_cuda_kv_cache_t* cache, const gi_cuda_attn_t* attn
 /* The cache of a model's decode steps: GI_TYPE_F32 (0, the default: the
  * rolling float32 cache), GI_TYPE_F16 or GI_TYPE_Q8_0 (half, or a quarter
  * and a sixteenth, of its size), written and read by the calls above
- * (kvcache.go's cache types).  Changing the type empties the cache; the step
- * is captured again at the next generate.  -2 for another type, while the
- * persistent layers are on, or under tensor parallelism; -4 for a head dim that gi_cuda_attn_dev does not
- * take. */
+ * (kvcache.go's cache types).  The call empties the cache, also when the type
+ * is the one it has; the step is captured again at the next generate.  -2 for
+ * another type, while the persistent layers are on, or under tensor
+ * parallelism; -4 for a head dim that gi_cuda_attn_dev does not take. */
 int gi_cuda_model_set_kv_cache(gi_cuda_model_t model, int type);
 
 /* The next token of each of `rows` rows of logits (vocab values each,
