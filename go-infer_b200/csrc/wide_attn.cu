@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
       }
       const int seen = seen_by(p, s_unit->s, (s_unit->row0 + min(r, s_unit->n_rows - 1)) / group) - s_unit->tile0 * kTok;
       const int seen_first = s_unit->seen_first - s_unit->tile0 * kTok;  // positions from the first tile's on
-      float o[kOut], m = -INFINITY, l = 0.f, alpha = 0.f;
+      float o[kOut], m = -INFINITY, l = 0.f, alpha = 0.f;  // m: of the products, before the factor
 #pragma unroll
       for (int i = 0; i < kOut; ++i) o[i] = 0.f;
       // A wait that gave up is taken to the next vote: no warp leaves on its own, and
@@ -571,10 +571,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
           s_max[((n & 1) * 2 + half) * kRows + r] = top;
           if (!(ok = soft_vote(ok))) break;
           top = fmaxf(top, s_max[((n & 1) * 2 + (half ^ 1)) * kRows + r]);
-          const float mn = top == -INFINITY ? m : fmaxf(m, top * fac);
-          zero = mn == -INFINITY ? 0.f : mn;
-          alpha_n = exp2_approx(m - zero);
-          m = mn;
+          top = fmaxf(m, top);
+          zero = top == -INFINITY ? 0.f : top;
+          alpha_n = m == -INFINITY ? 0.f : exp2_approx((m - zero) * fac);
+          m = top;
         }
         if (i > 0) {  // o = o alpha + P V of the tile before, before this tile's P lets the next one begin
           const int n = tile_no + i - 1;
@@ -592,16 +592,17 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
         }
         if (i < tiles) {
           float sum = 0.f, sum2 = 0.f;
-          // P at most 2^14, by a product, which rounds nothing.  Inside the exponent the power would save 4 of
-          // 291 us (7 chunks of 512 on up to 4000 positions) but have the sum rounded: 2^-21 of a weight, and half a
-          // step of 14 - zero where that is past a power of two (2^-12 with a maximum of -4090, 2^-8 with -65530).
+          // The maximum is taken off before the factor, so the largest weight is 1 exactly, however large the
+          // scores are: x fac - zero fac in one FMA leaves the rounding of zero fac, which is past half's range
+          // from scores of 2^25 on.  P at most 2^14, by a product, which rounds nothing; inside the exponent the
+          // power would be rounded to 2^-21 of a weight.
 #pragma unroll 1
           for (int j = 0; j < 64; j += 16) {
             float x[16];
             uint32_t w[16];
             tmem_ld16(s + j, x);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = exp2_approx(fmaf(x[e], fac, -zero)) * 16384.f;
+            for (int e = 0; e < 16; ++e) x[e] = exp2_approx((x[e] - zero) * fac) * 16384.f;
             if (masked) {
               const int l0 = limit(j);
 #pragma unroll
@@ -631,21 +632,25 @@ __global__ void __launch_bounds__(kWideThreads, 1) wide_kernel(KvCache c, Pass p
       // ---- the row: finished, its sums, or a part ----
       s_ml[half * kRows + r] = make_float2(m, l);
       if (!(ok = soft_vote(ok))) break;
-      const float sum = l + s_ml[(half ^ 1) * kRows + r].y;
+      float sum = l + s_ml[(half ^ 1) * kRows + r].y;
       const int row = s_unit->row0 + r;
       const bool real = r < s_unit->n_rows;
       const size_t at =
           (size_t)(s_unit->s.start + row / group) * p.n_heads + (size_t)s_unit->h * group + row % group;
-      float f = 1.f;
+      // What is joined with other parts is for the maximum in powers of two, m fac rounded: 2^(what was rounded off)
+      // goes to the sums, unless it is more than they bear (then scores are whole steps of 32 and more apart).
+      const float m2 = m == -INFINITY ? m : m * fac, rest = fmaf(m, fac, -m2);
+      float f = fabsf(rest) <= 16.f ? exp2f(rest) : 1.f;
+      sum *= f;
       float* out = p.out + at * HD + half * kOut;
       if (!s_unit->whole) {
         float* part = p.parts + (size_t)(2 * blockIdx.x + (s_unit->tile0 > 0 ? 0 : 1)) * W::kPart;
         out = part + r * HD + half * kOut;
-        if (half == 0 && real) *reinterpret_cast<float2*>(part + kRows * HD + 2 * r) = make_float2(m, sum);
+        if (half == 0 && real) *reinterpret_cast<float2*>(part + kRows * HD + 2 * r) = make_float2(m2, sum);
       } else if (p.ml) {
-        if (half == 0 && real) p.ml[at] = make_float2(m, sum);
+        if (half == 0 && real) p.ml[at] = make_float2(m2, sum);
       } else {
-        f = sum > 0.f ? 1.f / sum : 0.f;
+        f = sum > 0.f ? f / sum : 0.f;
       }
       if (real) {
 #pragma unroll
@@ -678,7 +683,7 @@ bool prepare_wide() {
 
 namespace paged {
 
-// Head dim 128 from 48 rows on: 4 sequences of 8000 positions, 8 kv heads, Q8_0, take 54 / 55 / 56 / 96 us here
+// Head dim 128 from 48 rows on: 4 sequences of 8000 positions, 8 kv heads, Q8_0, take 54 / 55 / 56 / 97 us here
 // with 48 / 64 / 96 / 256 rows per unit, and 63 / 58 / 65 / 211 us in units of at most 32 rows (paged_attn.cu); a
 // prefix of 8192 under 48 / 64 sequences 35 / 39 and 41 / 45 us.  Sequences of 500 positions lose up to 2 us by it
 // (48 rows: 20.7 against 18.2).  Head dim 64, half the work per tile, from 64 rows on: 47 against 51 us with 64

@@ -531,6 +531,53 @@ def test_attention_of_many_rows_of_any_magnitude(kind, dim, size):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,new", [(64, 1), (64, 40), (128, 1), (128, 40)])
+@pytest.mark.parametrize("prefix", [0, 150])
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 22, 2.0 ** 30, -2.0 ** 40, 2.0 ** 100])
+def test_attention_of_scores_far_beyond_one_step(kind, dim, new, prefix, size):
+    """One position's score is larger than every other's by far more than the exponent's range, and the scores
+    themselves are so large that a step of them in float32 is: the row is that position's V."""
+    n = 190
+    c = AttnCase(49, kind, 8, 2, dim, 16, [n, n], [new] * 2, prefix=prefix)
+    rng = np.random.default_rng(50)
+    c.cache.k[:] = 0
+    for x in (c.cache.ks, c.cache.vs):
+        if x is not None:
+            x[:] = 1
+    v = rng.integers(-60, 60, c.cache.v.shape)
+    c.cache.v[:] = v
+    k0 = rng.permutation(201)[:n] - 100  # of the own positions; the prefix's lie below or among them
+    p = np.arange(n)
+    for b in range(2):
+        c.cache.k[c.table[b, p // 16], :, p % 16, 0] = k0[:, None]
+    if prefix:
+        p = np.arange(prefix)
+        kp = rng.integers(-120, 121, prefix) // 2 * 2 + 0.5 if kind == G.TYPE_F16 else rng.integers(-126, -100, prefix)
+        c.cache.k[c.prefix_pages[p // 16], :, p % 16, 0] = kp[:, None]
+    c.q[:] = 0
+    c.q[..., 0] = size
+    c.data.copy_(dev(c.cache.data)), c.d["q"].copy_(dev(c.q))
+    torch.cuda.synchronize()
+    c.call()
+    c.stream.synchronize()
+    got = c.out.cpu().numpy().reshape(2, new, 8, dim)
+    sign = 1 if size > 0 else -1
+    for b in range(2):
+        for j in range(new):
+            seen = n - new + j + 1
+            score = sign * k0[:seen].astype(float)
+            at = int(score.argmax())
+            page, o = c.table[b, at // 16], at % 16
+            if prefix and (sign * kp).max() > score[at]:
+                best = np.flatnonzero(sign * kp == (sign * kp).max())
+                want = np.mean([c.cache.v[c.prefix_pages[i // 16], :, i % 16].astype(float) for i in best], axis=0)
+            else:
+                want = c.cache.v[page, :, o].astype(float)
+            # equal scores weigh the same to the exponent's 2^-22, the split and the sums round below 2^-18
+            assert np.abs(got[b, j] - np.repeat(want, 4, axis=0)).max() <= 60 * 2.0 ** -18
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("heads,kv,lens,new,prefix", [
     (3, 1, [150, 70], [97, 2], 0), (6, 2, [40, 200, 9], [12, 1, 3], 0), (4, 4, [0, 30, 90], None, 170), (12, 1, [60, 33], [9, 4], 250)])
 def test_attention_of_head_dim_96(kind, heads, kv, lens, new, prefix):
